@@ -103,7 +103,7 @@ def build_oracle(verbose: bool = False) -> None:
     _run(["make", "-s", "-C", oracle, "all"], verbose)
     # the reference tree: $TQK_REFERENCE, else a "reference" directory beside the repository
     ref = os.environ.get("TQK_REFERENCE") or os.path.join(os.path.dirname(ROOT), "reference")
-    if os.path.isdir(ref):
+    if os.path.exists(os.path.join(ref, "kernel", "quant_x.c")):
         _run(["make", "-s", "-C", oracle, f"REF={ref}", "ref"], verbose)
         if os.path.exists(os.path.join(PKG, "libtq_attn_b200.so")):
             _run(["make", "-s", "-C", oracle, f"REF={ref}", "_ref/test_model_dropin", "_ref/libtqref_dropin.so"],
