@@ -332,7 +332,7 @@ class Oracle:
 
     def forward_tokens(self, model: dict, tokens, max_tokens: int, start_planes=None):
         """The reference's own tq_ctx_init + tq_forward_token (model/context.c:6-122) over `tokens`
-        with a Q8 KV cache (reference builds only).  model: cfg (n_q_heads, n_kv_heads, head_dim,
+        with a Q8 KV cache; the port composes the restated steps.  model: cfg (n_q_heads, n_kv_heads, head_dim,
         hidden_size, rope_theta, rms_eps, n_layers, intermediate_size, vocab_size), fmt ("8" / "4"),
         embed (packed rows), final_norm, and layers: dicts with input_norm, post_norm, q_norm, k_norm
         and the packed wq, wk, wv, wo, wgate, wup, wdown.  Returns (logits per token [n][vocab],
@@ -340,7 +340,7 @@ class Oracle:
         [(k, v) per layer]) to start from a cache that already holds positions [0, pos) (copied into
         the context's planes) instead of an empty one."""
         if self.kind == "port":
-            raise ValueError("forward_tokens runs the reference's own runtime: a reference build is needed")
+            return self._port_forward_tokens(model, tokens, max_tokens, start_planes)
         c = model["cfg"]
         f = 0 if model["fmt"] == "8" else 1
         hidden, inter, vocab, hd = c["hidden_size"], c["intermediate_size"], c["vocab_size"], c["head_dim"]
@@ -402,6 +402,55 @@ class Oracle:
             return np.stack(logits), rcs, planes
         finally:
             self.lib.tq_ctx_free(ctypes.byref(ctx))
+
+    def _port_forward_tokens(self, model: dict, tokens, max_tokens: int, start_planes):
+        """forward_tokens from the restated steps (model/context.c:83-122, mlp.c:3-17, embedding.c:4-41)."""
+        c, fmt = model["cfg"], model["fmt"]
+        hidden, inter, vocab, eps = c["hidden_size"], c["intermediate_size"], c["vocab_size"], c["rms_eps"]
+        n_q, n_kv, hd = c["n_q_heads"], c["n_kv_heads"], c["head_dim"]
+        pos, planes0 = start_planes if start_planes is not None else (0, None)
+        row = hd // QK * BLOCK_BYTES
+        planes = [tuple(np.ascontiguousarray(p).reshape(n_kv, max_tokens, row).copy() for p in kv) for kv in planes0] \
+            if planes0 is not None else [tuple(np.zeros((n_kv, max_tokens, row), np.uint8) for _ in range(2))
+                                         for _ in range(c["n_layers"])]
+
+        def rmsnorm(x, w):
+            out = np.empty(hidden, np.float32)
+            self._fn["rmsnorm"](_vp(x), _vp(np.ascontiguousarray(w, dtype=np.float32)), _vp(out), hidden, eps)
+            return out
+
+        def matmul(w, x, rows, cols):
+            return self.matmul(w, fmt, self.quantize_rows(x[None])[0], rows, cols)
+
+        def embedding(token):
+            blocks = np.ascontiguousarray(model["embed"]).reshape(vocab, hidden // QK, -1)[token]
+            d = blocks[:, :4].copy().view(np.float32)
+            if fmt == "8":
+                q = blocks[:, 4:].view(np.int8)
+            else:
+                q = np.concatenate([blocks[:, 4:] & 15, blocks[:, 4:] >> 4], 1).astype(np.int32) - 8
+            return (d * q.astype(np.float32)).reshape(hidden)
+
+        logits, rcs = [], []
+        for t in tokens:
+            if pos >= max_tokens or not 0 <= int(t) < vocab:
+                rcs.append(-1)
+                logits.append(logits[-1] if logits else np.zeros(vocab, np.float32))
+                continue
+            x = embedding(int(t))
+            for lw, (kp, vp) in zip(model["layers"], planes):
+                xn = rmsnorm(x, lw["input_norm"])
+                x = x + self.attention_layer(lw, fmt, lw["q_norm"], lw["k_norm"], n_q, n_kv, hd, hidden,
+                                             c["rope_theta"], eps, kp, vp, max_tokens, pos, xn)
+                xn = rmsnorm(x, lw["post_norm"])
+                gate, up = matmul(lw["wgate"], xn, inter, hidden), matmul(lw["wup"], xn, inter, hidden)
+                with np.errstate(over="ignore"):
+                    act = gate * (np.float32(1) / (np.float32(1) + np.exp(-gate))) * up
+                x = x + matmul(lw["wdown"], act, hidden, inter)
+            logits.append(matmul(model["embed"], rmsnorm(x, model["final_norm"]), vocab, hidden))
+            rcs.append(0)
+            pos += 1
+        return np.stack(logits), rcs, planes
 
     def max_threads(self) -> int:
         return self.lib.refdrv_max_threads() if self.kind != "port" else os.cpu_count() or 1
