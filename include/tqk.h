@@ -49,7 +49,7 @@ typedef void *tqk_stream_t; /* a cudaStream_t */
 #define TQK_ENODEV         -24  /* no usable CUDA device */
 #define TQK_ETIMEOUT       -25  /* a device-side bounded wait gave up (see tqk_device_status) */
 #define TQK_EUNSUPPORTED   -26  /* head_dim > 256 or another shape outside the kernels' range */
-#define TQK_EDEVLEN        -27  /* a length read from device memory was outside [0, max_tokens] (clamped) */
+#define TQK_EDEVLEN        -27  /* a length, offset or index read from device memory was out of range (clamped) */
 
 TQK_API const char *tqk_status_string(int status);
 /* Text of the last failure on the calling host thread ("" if none). */
@@ -69,7 +69,7 @@ TQK_API int tqk_device_status(int *device_error, int clear);
  * tqk_device_status(&v, 1). */
 TQK_API int tqk_device_status_async(int *host_dst, tqk_stream_t stream);
 /* The status code of a device error word value: TQK_OK for 0, TQK_ETIMEOUT for
- * a bounded wait that gave up, TQK_EDEVLEN for a clamped device length. */
+ * a bounded wait that gave up, TQK_EDEVLEN for a clamped device length, offset or index. */
 TQK_API int tqk_device_error_status(int device_error);
 
 /* ---------------------------------------------------------------------------
@@ -204,6 +204,79 @@ TQK_API int tqk_decode_workspace_size(const tqk_decode_args *a, size_t *bytes);
  * allocated on first use, whose tickets live apart from the partials. */
 TQK_API int tqk_workspace_init(void *workspace, size_t bytes, tqk_stream_t stream);
 TQK_API int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t workspace_bytes, tqk_stream_t stream);
+
+/* Decode attention that also counts how much each cached row is attended to
+ * (no counterpart in the reference): tqk_decode_q8, and for every row t of every
+ * kv head
+ *     weight_out[t] = weight[t] + sum over the head's q heads of softmax(scores)[t],
+ * the running sums tqk_evict_q8 decides by.  The row that a fused append (k_new,
+ * v_new) writes starts from 0, whatever the slot's sum was, and gets its position
+ * if the caller keeps positions.  Sums of slots from len_i on are left as they
+ * are.  Same arguments, planes, lengths, append, norm and RoPE as tqk_decode_q8;
+ * only normalised output.  The output agrees with tqk_decode_q8's within the
+ * decode tolerance, not bit for bit (its splits may merge in another unit).
+ * Results do not depend on the run: sums are added in a fixed order.
+ *   - Lengths read from the device are clamped to max_len here (the workspace
+ *     holds no more scores), reported as TQK_EDEVLEN.
+ *   - The workspace holds the decode's tickets and partials and one float per
+ *     q head and position: tqk_decode_weights_workspace_size() bytes, under
+ *     tqk_decode_q8's rules (zeroed once, ordered on one stream, shared with
+ *     tqk_decode_q8 if large enough); NULL = library-owned, per (device, stream).
+ *   - Two launches, capturable in a CUDA graph (with a caller workspace, or after
+ *     one earlier call on the same stream outside capture). */
+typedef struct {
+    const float *weight;         /* device, [n_kv][max_tokens] of item 0: the sums before the call */
+    float *weight_out;           /* device, same layout: the sums after it; may be weight (the usual case), else
+                                    must not overlap it */
+    int64_t item_stride;         /* elements between items' sums, and positions: at least n_kv * max_tokens
+                                    (ignored for one item) */
+    int32_t *position;           /* device, same layout, or NULL: the append writes the new token's position */
+    const int32_t *new_pos;      /* device [n_items]: the appended tokens' positions, or NULL: */
+    int new_pos0;                /* the one position of every item (the layers of one token) */
+} tqk_weights_args;
+TQK_API int tqk_decode_weights_workspace_size(const tqk_decode_args *a, size_t *bytes);
+TQK_API int tqk_decode_q8_weights(const tqk_decode_args *a, const tqk_weights_args *w, void *workspace,
+                                  size_t workspace_bytes, tqk_stream_t stream);
+
+/* Eviction from Q8 caches by accumulated attention weight (no counterpart in the
+ * reference).  In each (item, kv head) whose first len_i slots hold more than
+ * `budget` rows, `budget` rows are kept: first of all those whose position is
+ * below n_first or above newest - n_recent (newest: the head's largest position),
+ * then by falling weight; equal weights keep the lower slot, NaN ranks below every
+ * number, -0 equals +0.  Kept rows stay in their slots, except that the j-th kept
+ * row from slot `budget` on moves to the j-th evicted slot below it -- K, V, sum
+ * and position.  So rows move only as far as needed, and their order in the cache
+ * is no longer that of the positions; attention does not depend on it (RoPE is
+ * already in the K rows).  Afterwards the item has min(len_i, budget) rows
+ * (lens_out); a next token is appended at that slot with its own position's RoPE.
+ *   - Slots from min(len_i, budget) on are left as they were in every array.
+ *   - weight_out / position_out may be weight / position (in place) or arrays of
+ *     their own (which then receive every kept row's value); they must not
+ *     overlap otherwise.  lens_out may be lens.
+ *   - position may be NULL when n_first and n_recent are 0.
+ *   - max_len at most TQK_EVICT_MAX_LEN.  Device lengths are clamped to max_len
+ *     and reported as TQK_EDEVLEN.
+ *   - No workspace; one launch, and one more with lens_out. */
+#define TQK_EVICT_MAX_LEN 516096
+typedef struct {
+    tqk_block_q8 *k, *v;         /* planes of item 0 (device), [n_kv][max_tokens][head_dim/32] */
+    int64_t item_stride;         /* blocks between items' planes: at least n_kv * max_tokens * head_dim/32
+                                    (ignored for one item) */
+    int n_items, n_kv_heads, head_dim, max_tokens;
+    const int32_t *lens;         /* device [n_items], or NULL: */
+    int len0, len_step;          /* len_i = len0 + i * len_step */
+    int max_len;                 /* with lens: upper bound of len_i */
+    int budget;                  /* rows kept per head, 1 .. max_tokens */
+    int n_first, n_recent;       /* rows never evicted: n_first + n_recent <= budget */
+    const float *weight;         /* device [n_kv][max_tokens] of item 0 */
+    float *weight_out;
+    const int32_t *position;     /* device, same layout */
+    int32_t *position_out;
+    int64_t stat_item_stride;    /* elements between items' sums and positions: at least n_kv * max_tokens
+                                    (ignored for one item) */
+    int32_t *lens_out;           /* device [n_items], or NULL */
+} tqk_evict_args;
+TQK_API int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream);
 
 /* tqk_decode_q8 without any device allocation (no counterpart in the
  * reference): for callers that cannot allocate device memory at run time, for
@@ -355,6 +428,50 @@ TQK_API size_t tqk_forward_scratch_bytes(const tqk_model *m);
  * [0, vocab_size), before touching anything.  workspace: as tqk_decode_q8's. */
 TQK_API int tqk_forward_token(const tqk_model *m, int token, int pos, void *scratch, float *logits,
                               int32_t *next_token, void *workspace, size_t workspace_bytes, tqk_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Constraints on the next token (no counterpart in the reference): penalties for
+ * the tokens a sequence already has, token biases and a grammar's bit mask, and
+ * the greedy choice among what is left.  For each row r and token t, in this order:
+ *   seen in the row's history:       x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   seen n > 0 times after the history's first prompt_lens[r] tokens:
+ *                                    x = (x - frequency[r] * n) - presence[r]
+ *   in the row's bias list:          x = x + (the sum of its values there, in list order)
+ *   bit t of the row's mask clear:   x = -inf, whatever it was
+ * each step rounded to fp32.  choice[r] is the first token of the largest x (as
+ * sample_greedy, reference model/sampler.c:3-13, but NaN is never chosen), or -1
+ * when nothing above -inf is left.
+ *   - Histories and bias lists are packed: row r's are entries offsets[r] ..
+ *     offsets[r + 1] - 1.  Entries outside [0, vocab_size) are skipped; an offset
+ *     outside [0, n_tokens] / [0, n_bias], or falling, is clamped and reported as
+ *     TQK_EDEVLEN.  prompt_lens is clamped to the history's length.
+ *   - mask: word t / 32, bit t % 32 allows token t.  mask_rows[r] is the mask row
+ *     of row r, -1 for no mask; an index from n_mask_rows on (or below -1) allows
+ *     nothing and is reported as TQK_EDEVLEN.
+ *   - out may be logits (same stride) and must not overlap it otherwise; NULL =
+ *     only the choice.  One launch, no workspace. */
+typedef struct {
+    const float *logits;            /* device [n_rows][vocab_size] */
+    int64_t logits_stride;          /* floats between rows (0 = vocab_size) */
+    float *out;                     /* device, or NULL */
+    int64_t out_stride;             /* (0 = vocab_size) */
+    int32_t *choice;                /* device [n_rows], or NULL */
+    int n_rows, vocab_size;
+    const int32_t *tokens;          /* device [n_tokens] histories, or NULL (then no penalties) */
+    const int32_t *token_offsets;   /* device [n_rows + 1] */
+    int n_tokens;
+    const int32_t *prompt_lens;     /* device [n_rows], or NULL = 0 */
+    const float *repetition, *frequency, *presence;  /* device [n_rows] each, NULL = off; repetition > 0 */
+    const int32_t *bias_tokens;     /* device [n_bias], or NULL */
+    const float *bias_values;       /* device [n_bias] */
+    const int32_t *bias_offsets;    /* device [n_rows + 1] */
+    int n_bias;
+    const uint32_t *mask;           /* device [n_mask_rows][mask_stride], or NULL */
+    int64_t mask_stride;            /* words between mask rows (0 = ceil(vocab_size / 32)) */
+    const int32_t *mask_rows;       /* device [n_rows], or NULL = row r */
+    int n_mask_rows;                /* (without mask_rows: at least n_rows) */
+} tqk_logits_args;
+TQK_API int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream);
 
 /* attend_q8 for one layer of one sequence: n = pos + 1 positions
  * (reference model/attention_layer.c:125-150); TQK_EPOS if pos is out of range. */

@@ -23,14 +23,14 @@ INCLUDE = os.path.join(ROOT, "include")
 
 CUDA_SOURCES = ["tqk_runtime.cu", "tqk_quant.cu", "tqk_decode.cu", "tqk_prefill.cu", "tqk_prologue.cu",
                 "tqk_matvec.cu", "tqk_layer.cu", "tqk_pack.cu", "tqk_ref_ops.cu", "tqk_exchange.cu",
-                "tqk_forward.cu", "tqk_inputs.cu"]
+                "tqk_forward.cu", "tqk_inputs.cu", "tqk_evict.cu", "tqk_logits.cu"]
 DROPIN_SOURCES = ["dropin/tq_attn_b200.c"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "-Xptxas", "-warn-spills",
+    "-Xptxas", "-warn-spills", "--threads", "0",
 ]
 
 HOST_CC = "/usr/bin/gcc"  # the image's $CC (/opt/gcc) lacks libgomp

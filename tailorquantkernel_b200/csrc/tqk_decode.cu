@@ -91,7 +91,32 @@ struct DecodeParams {
     // the packed kernel's split merge through a thread-block cluster (the max_splits CTAs of one
     // unit, cluster dims (cluster, 1, 1)); 0 = tickets and partials in global memory
     int cluster;
+    // attention-weight sums (tqk_decode_q8_weights; kernels with WT != WT_NONE): every score of the call goes
+    // to scores [item][q head][score_stride] and each q head's final running max and sum to ml [item][q head].
+    // Lengths are clamped to len_cap (the call's max_len: the scores buffer holds no more)
+    float *scores;
+    long long score_stride;
+    float2 *ml;
+    int len_cap;
 };
+
+// What a kernel hands to the weight pass of tqk_decode_q8_weights: nothing, scores and maxima in natural
+// units, or in log2 units (the tensor-core kernels, whose softmax is base 2).  In log2 units the split
+// merges stay base 2 as well, so that a weight 2^(s - m) / l refers to the very max its l was summed under.
+enum : int { WT_NONE = 0, WT_NAT = 1, WT_LOG2 = 2 };
+
+// Where q head qh's scores of `item` start.
+__device__ __forceinline__ float *score_row_of(const DecodeParams &p, int item, int qh) {
+    return p.scores + ((long long)item * (p.n_kv * p.group) + qh) * p.score_stride;
+}
+// Clamped length of an item; records lengths outside [0, cap].
+__device__ __forceinline__ int clamp_len(const DecodeParams &p, int len, int cap, bool report) {
+    if (len < 0 || len > cap) {
+        if (report) record_error(p.err, DEVERR_BADLEN);
+        len = len < 0 ? 0 : cap;
+    }
+    return len;
+}
 
 // One element of the call's normalised output: head qh (of the item) column c.
 template <int HD>
@@ -239,7 +264,7 @@ __device__ __forceinline__ bool last_arrival(int *ticket, int n, int tid, int *f
 // slots.  The loads are the latency: the accumulators of up to KB slots are
 // loaded in one batch, the first batch together with every slot's (m, l), so
 // a merge of up to KB slots costs one L2 round trip.
-template <int HD, int GROWS, int NT, int BAR>
+template <int HD, int GROWS, int NT, int BAR, int WT>
 __device__ __forceinline__ void merge_slots(const DecodeParams &p, float *pb, int first, int stride, int n, int G,
                                             int tid, float *wts, float *ms, float *ls, bool to_part, float *out_item,
                                             int item, int qh0) {
@@ -276,7 +301,8 @@ __device__ __forceinline__ void merge_slots(const DecodeParams &p, float *pb, in
         M = warp_max(M);
         float Lsum = 0.0f;
         for (int k = lane; k < n; k += 32) {
-            const float w = expf(wts[k * GROWS + g] - M);
+            const float d = wts[k * GROWS + g] - M;
+            const float w = WT == WT_LOG2 ? exp2f(d) : expf(d);
             wts[k * GROWS + g] = w;
             Lsum += lall[k * GROWS + g] * w;
         }
@@ -310,6 +336,8 @@ __device__ __forceinline__ void merge_slots(const DecodeParams &p, float *pb, in
             if (c == 0) { d[HD] = ms[g]; d[HD + 1] = ls[g]; }
         } else if (p.out_mode == TQK_OUT_NORMALIZED) {
             store_out<HD>(p, out_item, item, qh0 + g, c, a[e] / ls[g]);
+            if (WT != WT_NONE && c == 0)
+                p.ml[(long long)item * (p.n_kv * p.group) + qh0 + g] = make_float2(ms[g], ls[g]);
         } else {
             float *o = out_item + (long long)(qh0 + g) * RS;
             o[c] = a[e];
@@ -331,7 +359,7 @@ __device__ __forceinline__ void merge_slots(const DecodeParams &p, float *pb, in
 // overwritten by the merge; the tickets used are left at zero.
 // pb: the unit's partial slots ([slot][GROWS][HD + 2] floats); tickets: its
 // ticket block ([0] final, [1 + i] group i).
-template <int HD, int GROWS, int NT, int BAR, typename AccFn>
+template <int HD, int GROWS, int NT, int BAR, int WT, typename AccFn>
 __device__ __forceinline__ void finish_split_at(const DecodeParams &p, int tid, float *pb, int *tickets, int s,
                                                 int n_splits, int item, int qh0, int G, float *out_item, AccFn acc,
                                                 float *ms, float *ls, float *wts, int *flag) {
@@ -342,6 +370,8 @@ __device__ __forceinline__ void finish_split_at(const DecodeParams &p, int tid, 
         if (single) {
             if (p.out_mode == TQK_OUT_NORMALIZED) {
                 store_out<HD>(p, out_item, item, qh0 + g, c, a / ls[g]);
+                if (WT != WT_NONE && c == 0)
+                    p.ml[(long long)item * (p.n_kv * p.group) + qh0 + g] = make_float2(ms[g], ls[g]);
             } else {
                 float *o = out_item + (long long)(qh0 + g) * (HD + 2);
                 o[c] = a;
@@ -359,32 +389,32 @@ __device__ __forceinline__ void finish_split_at(const DecodeParams &p, int tid, 
         const int gi = s / MERGE_GROUP, first = gi * MERGE_GROUP;
         const int gsz = min(MERGE_GROUP, n_splits - first);
         if (!last_arrival<BAR, NT>(tickets + 1 + gi, gsz, tid, flag)) return;
-        merge_slots<HD, GROWS, NT, BAR>(p, pb, first, 1, gsz, G, tid, wts, ms, ls, true, out_item, item, qh0);
+        merge_slots<HD, GROWS, NT, BAR, WT>(p, pb, first, 1, gsz, G, tid, wts, ms, ls, true, out_item, item, qh0);
         if (tid == 0) tickets[1 + gi] = 0;
         const int n_groups = (n_splits + MERGE_GROUP - 1) / MERGE_GROUP;
         if (!last_arrival<BAR, NT>(tickets, n_groups, tid, flag)) return;
-        merge_slots<HD, GROWS, NT, BAR>(p, pb, 0, MERGE_GROUP, n_groups, G, tid, wts, ms, ls, false, out_item, item,
-                                        qh0);
+        merge_slots<HD, GROWS, NT, BAR, WT>(p, pb, 0, MERGE_GROUP, n_groups, G, tid, wts, ms, ls, false, out_item,
+                                            item, qh0);
     } else {
         if (!last_arrival<BAR, NT>(tickets, n_splits, tid, flag)) return;
-        merge_slots<HD, GROWS, NT, BAR>(p, pb, 0, 1, n_splits, G, tid, wts, ms, ls, false, out_item, item, qh0);
+        merge_slots<HD, GROWS, NT, BAR, WT>(p, pb, 0, 1, n_splits, G, tid, wts, ms, ls, false, out_item, item, qh0);
     }
     if (tid == 0) tickets[0] = 0;  // ready for the next launch
 }
 
 // The fixed-split layout: unit (item, pair) owns max_splits slots and
 // TICKETS_PER_UNIT tickets.
-template <int HD, int GROWS, int NT, int BAR, typename AccFn>
+template <int HD, int GROWS, int NT, int BAR, int WT, typename AccFn>
 __device__ __forceinline__ void finish_split(const DecodeParams &p, int tid, int item, int pair, int s, int n_splits,
                                              int qh0, int G, float *out_item, AccFn acc, float *ms, float *ls,
                                              float *wts, int *flag) {
     const long long unit = (long long)item * p.pairs + pair;
-    finish_split_at<HD, GROWS, NT, BAR>(p, tid, p.part + unit * p.max_splits * GROWS * (HD + 2),
-                                        p.counters + unit * TICKETS_PER_UNIT, s, n_splits, item, qh0, G, out_item, acc,
-                                        ms, ls, wts, flag);
+    finish_split_at<HD, GROWS, NT, BAR, WT>(p, tid, p.part + unit * p.max_splits * GROWS * (HD + 2),
+                                            p.counters + unit * TICKETS_PER_UNIT, s, n_splits, item, qh0, G, out_item,
+                                            acc, ms, ls, wts, flag);
 }
 
-template <int NB, int GMAX>
+template <int NB, int GMAX, int WT>
 __global__ void __launch_bounds__(DEC_THREADS) decode_q8_kernel(const DecodeParams p) {
     using L = DecLayout<NB, GMAX>;
     constexpr int HD = L::HD, ROW = L::ROW, STAGES = L::STAGES;
@@ -407,11 +437,8 @@ __global__ void __launch_bounds__(DEC_THREADS) decode_q8_kernel(const DecodePara
     const int slice = pair - kvh * p.head_slices;
     const int g0 = slice * p.heads_per_cta;
     const int G = min(p.heads_per_cta, p.group - g0);
-    int len = p.lens ? p.lens[item] : p.len0 + item * p.len_step;
-    if (len < 0 || len > p.max_tokens) {
-        if (tid == 0) record_error(p.err, DEVERR_BADLEN);
-        len = len < 0 ? 0 : p.max_tokens;
-    }
+    const int len = clamp_len(p, p.lens ? p.lens[item] : p.len0 + item * p.len_step,
+                              WT != WT_NONE ? p.len_cap : p.max_tokens, tid == 0);
     int n_splits = n_splits_of(len, p.split_tokens);
     if (n_splits > p.max_splits) {  // a device length above the max_len the grid was sized for
         if (tid == 0) record_error(p.err, DEVERR_BADLEN);
@@ -596,7 +623,10 @@ __global__ void __launch_bounds__(DEC_THREADS) decode_q8_kernel(const DecodePara
         for (int it = tid; it < DEC_T * GMAX; it += DEC_THREADS) {
             const int tt = it / GMAX;
             float sv = -INFINITY;
-            if (gq < G && tt < rows) sv = score_row<NB>(ks + tt * ROW, qw, qds, p.scale);
+            if (gq < G && tt < rows) {
+                sv = score_row<NB>(ks + tt * ROW, qw, qds, p.scale);
+                if constexpr (WT != WT_NONE) score_row_of(p, item, qh0 + gq)[t0 + tt] = sv;
+            }
             sc[gq * DEC_T + tt] = sv;
         }
         if (!__syncthreads_and(ok)) {
@@ -695,14 +725,15 @@ __global__ void __launch_bounds__(DEC_THREADS) decode_q8_kernel(const DecodePara
         for (int w = 0; w < DEC_WARPS; w++) a += red[(w * GMAX + g) * HD + c];
         return a;
     };
-    finish_split<HD, GMAX, DEC_THREADS, 0>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, m_s, l_s,
-                                          red + DEC_WARPS * GMAX * HD, flag);
+    finish_split<HD, GMAX, DEC_THREADS, 0, WT>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, m_s, l_s,
+                                              red + DEC_WARPS * GMAX * HD, flag);
 }
 
 }  // namespace tqk
 
 #include "tqk_decode_mma.cuh"
 #include "tqk_decode_pack.cuh"
+#include "tqk_decode_weights.cuh"
 
 namespace tqk {
 
@@ -744,7 +775,7 @@ namespace {
 int gmax_for(int group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
 
 // Tensor-core kernel (head_dim 128 / 256): up to 16 q heads per CTA.
-template <int NB, int GPAD>
+template <int NB, int GPAD, int WT>
 int launch_mma(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas_per_sm) {
     using L = MmaLayout<NB, GPAD>;
     static std::mutex mu;
@@ -756,11 +787,11 @@ int launch_mma(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas_
     {
         std::lock_guard<std::mutex> lock(mu);
         if (occ_by_dev[dev] == 0) {
-            e = cudaFuncSetAttribute(decode_q8_mma_kernel<NB, GPAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(decode_q8_mma_kernel<NB, GPAD, WT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      L::BYTES);
             int o = 0;
             if (e == cudaSuccess)
-                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_mma_kernel<NB, GPAD>, MMA_THREADS,
+                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_mma_kernel<NB, GPAD, WT>, MMA_THREADS,
                                                                   L::BYTES);
             if (e != cudaSuccess) return fail_cuda(e, "decode_q8_mma_kernel attributes");
             occ_by_dev[dev] = o > 0 ? o : -1;
@@ -771,15 +802,16 @@ int launch_mma(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas_
         *ctas_per_sm = occ;
         return TQK_OK;
     }
-    return launch_pdl(decode_q8_mma_kernel<NB, GPAD>, grid, dim3(MMA_THREADS), L::BYTES, stream, p);
+    return launch_pdl(decode_q8_mma_kernel<NB, GPAD, WT>, grid, dim3(MMA_THREADS), L::BYTES, stream, p);
 }
 
 // Two-kv-heads-per-CTA kernel for 4 q heads per kv head.
 // How many clusters of cx CTAs of `kernel` the device `dev` holds at once (cached per device and
 // cluster size; sizes above 8 are opted in as non-portable); 0 when it holds none, or with
-// TQK_DECODE_CLUSTER=0 in the environment.
-template <typename K>
-int max_active_clusters(K kernel, int dev, unsigned cx, int threads, int smem) {
+// TQK_DECODE_CLUSTER=0 in the environment.  The kernel is a template argument: kernels of one type
+// each have a cache, and an opt-in, of their own.
+template <auto kernel>
+int max_active_clusters(int dev, unsigned cx, int threads, int smem) {
     static std::mutex mu;
     static int count_by[64][CL_MAX + 1];  // 0 = unknown, -1 = none, n = n clusters
     static const bool enabled = [] {
@@ -813,7 +845,7 @@ int max_active_clusters(K kernel, int dev, unsigned cx, int threads, int smem) {
     return count > 0 ? count : 0;
 }
 
-template <int NB>
+template <int NB, int WT>
 int launch_pack(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas_per_sm) {
     using L = PackLayout<NB>;
     static std::mutex mu;
@@ -825,10 +857,10 @@ int launch_pack(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas
     {
         std::lock_guard<std::mutex> lock(mu);
         if (occ_by_dev[dev] == 0) {
-            e = cudaFuncSetAttribute(decode_q8_pack_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+            e = cudaFuncSetAttribute(decode_q8_pack_kernel<NB, WT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
             int o = 0;
             if (e == cudaSuccess)
-                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_pack_kernel<NB>, PK_THREADS, L::BYTES);
+                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_pack_kernel<NB, WT>, PK_THREADS, L::BYTES);
             if (e != cudaSuccess) return fail_cuda(e, "decode_q8_pack_kernel attributes");
             occ_by_dev[dev] = o > 0 ? o : -1;
         }
@@ -847,16 +879,16 @@ int launch_pack(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas
     const bool equal_lengths = p.lens == nullptr && p.len_step == 0;
     if (equal_lengths && grid.x >= 2 && grid.x <= (unsigned)CL_MAX &&
         (long long)grid.y * grid.z <=
-            max_active_clusters(decode_q8_pack_kernel<NB>, dev, grid.x, PK_THREADS, L::BYTES)) {
+            max_active_clusters<decode_q8_pack_kernel<NB, WT>>(dev, grid.x, PK_THREADS, L::BYTES)) {
         DecodeParams pc = p;
         pc.cluster = (int)grid.x;
-        return launch_pdl_cluster(decode_q8_pack_kernel<NB>, grid, dim3(PK_THREADS), L::BYTES, stream, grid.x, pc);
+        return launch_pdl_cluster(decode_q8_pack_kernel<NB, WT>, grid, dim3(PK_THREADS), L::BYTES, stream, grid.x, pc);
     }
-    return launch_pdl(decode_q8_pack_kernel<NB>, grid, dim3(PK_THREADS), L::BYTES, stream, p);
+    return launch_pdl(decode_q8_pack_kernel<NB, WT>, grid, dim3(PK_THREADS), L::BYTES, stream, p);
 }
 
 // The balanced (stream-K) schedule of the same kernel: a 1-D grid of equal tile runs.
-template <int NB>
+template <int NB, int WT>
 int launch_pack_bal(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas_per_sm) {
     using L = PackBalLayout<NB>;
     static std::mutex mu;
@@ -868,11 +900,11 @@ int launch_pack_bal(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *
     {
         std::lock_guard<std::mutex> lock(mu);
         if (occ_by_dev[dev] == 0) {
-            e = cudaFuncSetAttribute(decode_q8_pack_bal_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(decode_q8_pack_bal_kernel<NB, WT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      L::BYTES);
             int o = 0;
             if (e == cudaSuccess)
-                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_pack_bal_kernel<NB>, PK_THREADS,
+                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_pack_bal_kernel<NB, WT>, PK_THREADS,
                                                                   L::BYTES);
             if (e != cudaSuccess) return fail_cuda(e, "decode_q8_pack_bal_kernel attributes");
             occ_by_dev[dev] = o > 0 ? o : -1;
@@ -883,21 +915,26 @@ int launch_pack_bal(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *
         *ctas_per_sm = occ;
         return TQK_OK;
     }
-    return launch_pdl(decode_q8_pack_bal_kernel<NB>, grid, dim3(PK_THREADS), L::BYTES, stream, p);
+    return launch_pdl(decode_q8_pack_bal_kernel<NB, WT>, grid, dim3(PK_THREADS), L::BYTES, stream, p);
 }
 
-int dispatch_pack(int nb, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ, bool balanced = false) {
-    if (nb == 4) return balanced ? launch_pack_bal<4>(p, grid, stream, occ) : launch_pack<4>(p, grid, stream, occ);
+template <int WT>
+int dispatch_pack_wt(int nb, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ, bool balanced) {
+    if (nb == 4)
+        return balanced ? launch_pack_bal<4, WT>(p, grid, stream, occ) : launch_pack<4, WT>(p, grid, stream, occ);
     return fail(TQK_EUNSUPPORTED, "decode: packed kernel needs head_dim 128");
 }
 
-int dispatch_mma(int nb, int gpad, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ) {
-    if (nb == 4) return gpad > 8 ? launch_mma<4, 16>(p, grid, stream, occ) : launch_mma<4, 8>(p, grid, stream, occ);
-    if (nb == 8) return gpad > 8 ? launch_mma<8, 16>(p, grid, stream, occ) : launch_mma<8, 8>(p, grid, stream, occ);
+template <int WT>
+int dispatch_mma_wt(int nb, int gpad, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ) {
+    if (nb == 4)
+        return gpad > 8 ? launch_mma<4, 16, WT>(p, grid, stream, occ) : launch_mma<4, 8, WT>(p, grid, stream, occ);
+    if (nb == 8)
+        return gpad > 8 ? launch_mma<8, 16, WT>(p, grid, stream, occ) : launch_mma<8, 8, WT>(p, grid, stream, occ);
     return fail(TQK_EUNSUPPORTED, "decode: tensor-core kernel needs head_dim 128 or 256");
 }
 
-template <int NB, int GMAX>
+template <int NB, int GMAX, int WT>
 int launch_decode(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ctas_per_sm) {
     using L = DecLayout<NB, GMAX>;
     // the dynamic shared-memory opt-in is a per-device function attribute
@@ -910,10 +947,10 @@ int launch_decode(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ct
     {
         std::lock_guard<std::mutex> lock(mu);
         if (occ_by_dev[dev] == 0) {
-            e = cudaFuncSetAttribute(decode_q8_kernel<NB, GMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+            e = cudaFuncSetAttribute(decode_q8_kernel<NB, GMAX, WT>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
             int o = 0;
             if (e == cudaSuccess)
-                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_kernel<NB, GMAX>, DEC_THREADS, L::BYTES);
+                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&o, decode_q8_kernel<NB, GMAX, WT>, DEC_THREADS, L::BYTES);
             if (e != cudaSuccess) return fail_cuda(e, "decode_q8_kernel attributes");
             occ_by_dev[dev] = o > 0 ? o : -1;
         }
@@ -923,24 +960,25 @@ int launch_decode(const DecodeParams &p, dim3 grid, cudaStream_t stream, int *ct
         *ctas_per_sm = occ;
         return TQK_OK;
     }
-    return launch_pdl(decode_q8_kernel<NB, GMAX>, grid, dim3(DEC_THREADS), L::BYTES, stream, p);
+    return launch_pdl(decode_q8_kernel<NB, GMAX, WT>, grid, dim3(DEC_THREADS), L::BYTES, stream, p);
 }
 
-template <int NB>
+template <int NB, int WT>
 int dispatch_gmax(int gmax, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ) {
     switch (gmax) {
-        case 1: return launch_decode<NB, 1>(p, grid, stream, occ);
-        case 2: return launch_decode<NB, 2>(p, grid, stream, occ);
-        case 4: return launch_decode<NB, 4>(p, grid, stream, occ);
-        default: return launch_decode<NB, 8>(p, grid, stream, occ);
+        case 1: return launch_decode<NB, 1, WT>(p, grid, stream, occ);
+        case 2: return launch_decode<NB, 2, WT>(p, grid, stream, occ);
+        case 4: return launch_decode<NB, 4, WT>(p, grid, stream, occ);
+        default: return launch_decode<NB, 8, WT>(p, grid, stream, occ);
     }
 }
 
 // CUDA-core kernel: head_dim 32 and 64 (128 and 256 go to the tensor-core kernels).
-int dispatch(int nb, int gmax, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ) {
+template <int WT>
+int dispatch_cuda_core(int nb, int gmax, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ) {
     switch (nb) {
-        case 1: return dispatch_gmax<1>(gmax, p, grid, stream, occ);
-        case 2: return dispatch_gmax<2>(gmax, p, grid, stream, occ);
+        case 1: return dispatch_gmax<1, WT>(gmax, p, grid, stream, occ);
+        case 2: return dispatch_gmax<2, WT>(gmax, p, grid, stream, occ);
         default: return fail(TQK_EUNSUPPORTED, "decode: the CUDA-core kernel takes head_dim 32 or 64");
     }
 }
@@ -949,6 +987,7 @@ struct Plan {
     int nb, gmax, heads_per_cta, head_slices, pairs, split_tokens, max_splits, max_len;
     bool mma;   // tensor-core kernel (head_dim 128/256) or the CUDA-core one (32/64)
     bool pack;  // tensor-core kernel with two kv heads per CTA (4 q heads per kv head)
+    bool weights;           // the call's scores go to the weight pass (tqk_decode_q8_weights)
     bool balanced;          // packed kernel on the balanced schedule: bal_ctas equal tile runs
     int bal_ctas, tickets_per_unit;
     size_t counters_bytes, part_bytes;
@@ -965,6 +1004,19 @@ size_t counters_region(int n_items, int units) {
     const size_t n = (size_t)n_items * units;
     const size_t b = ((n < TICKET_FLOOR_UNITS ? TICKET_FLOOR_UNITS : n) * TICKETS_PER_UNIT * sizeof(int) + 255) / 256 * 256;
     return b;
+}
+
+// Launches the plan's kernel (balanced: the packed kernel on the balanced schedule), or with occ != nullptr
+// only asks for its resident CTAs per SM.
+int dispatch(const Plan &pl, const DecodeParams &p, dim3 grid, cudaStream_t stream, int *occ, bool balanced = false) {
+    if (pl.pack)
+        return pl.weights ? dispatch_pack_wt<WT_LOG2>(pl.nb, p, grid, stream, occ, balanced)
+                          : dispatch_pack_wt<WT_NONE>(pl.nb, p, grid, stream, occ, balanced);
+    if (pl.mma)
+        return pl.weights ? dispatch_mma_wt<WT_LOG2>(pl.nb, pl.gmax, p, grid, stream, occ)
+                          : dispatch_mma_wt<WT_NONE>(pl.nb, pl.gmax, p, grid, stream, occ);
+    return pl.weights ? dispatch_cuda_core<WT_NAT>(pl.nb, pl.gmax, p, grid, stream, occ)
+                      : dispatch_cuda_core<WT_NONE>(pl.nb, pl.gmax, p, grid, stream, occ);
 }
 
 // K/V bytes a call streams with every item at max_len.
@@ -992,7 +1044,7 @@ long long auto_splits(bool uniform, long long slots, long long units, long long 
     return want < 1 ? 1 : want;
 }
 
-int make_plan(const tqk_decode_args *a, Plan *pl, bool gather = false) {
+int make_plan(const tqk_decode_args *a, Plan *pl, bool gather = false, bool weights = false) {
     if (!a) return fail(TQK_EINVAL, "decode: NULL args");
     if (a->n_items <= 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->head_dim <= 0 || a->max_tokens <= 0)
         return fail(TQK_EINVAL, "decode: non-positive shape");
@@ -1027,6 +1079,7 @@ int make_plan(const tqk_decode_args *a, Plan *pl, bool gather = false) {
     }
     const int group = a->n_q_heads / a->n_kv_heads;
     pl->nb = nb;
+    pl->weights = weights;
     pl->mma = nb % 4 == 0;
     pl->pack = nb == 4 && group == 4 && a->n_kv_heads % 2 == 0;  // head_dim 128 only (register budget)
     pl->gmax = pl->pack ? 8 : pl->mma ? (group <= 8 ? 8 : 16) : gmax_for(group);
@@ -1055,15 +1108,13 @@ int make_plan(const tqk_decode_args *a, Plan *pl, bool gather = false) {
         bool balanced = can_balance && (split == TQK_SPLIT_BALANCED || ragged);
         int occ = 0;
         DecodeParams dummy{};
-        int orc = pl->pack  ? dispatch_pack(nb, dummy, dim3(1), nullptr, &occ, balanced)
-                  : pl->mma ? dispatch_mma(nb, pl->gmax, dummy, dim3(1), nullptr, &occ)
-                            : dispatch(nb, pl->gmax, dummy, dim3(1), nullptr, &occ);
+        int orc = dispatch(*pl, dummy, dim3(1), nullptr, &occ, balanced);
         if (orc) return orc;
         long long slots = (long long)(d ? d->sm_count : 148) * (occ > 0 ? occ : 1);
         if (balanced && split != TQK_SPLIT_BALANCED &&
             pairs_total * ((max_len + PK_T - 1) / PK_T) < (long long)BAL_MIN_TILES * slots) {
             balanced = false;
-            orc = dispatch_pack(nb, dummy, dim3(1), nullptr, &occ, false);
+            orc = dispatch(*pl, dummy, dim3(1), nullptr, &occ);
             if (orc) return orc;
             slots = (long long)(d ? d->sm_count : 148) * (occ > 0 ? occ : 1);
         }
@@ -1199,14 +1250,123 @@ int decode_impl(const tqk_decode_args *a, const tqk_gather_dst *gd, void *worksp
         p.g_epoch = gd->epoch;
         for (int r = 0; r < gd->world; r++) p.g_out[r] = reinterpret_cast<uint2 *>(gd->out[r]);
     }
-    if (pl.balanced) return dispatch_pack(pl.nb, p, dim3((unsigned)pl.bal_ctas), st, nullptr, true);
+    if (pl.balanced) return dispatch(pl, p, dim3((unsigned)pl.bal_ctas), st, nullptr, true);
     const dim3 grid((unsigned)pl.max_splits, (unsigned)pl.pairs, (unsigned)a->n_items);
-    if (pl.pack) return dispatch_pack(pl.nb, p, grid, st, nullptr);
-    return pl.mma ? dispatch_mma(pl.nb, pl.gmax, p, grid, st, nullptr) : dispatch(pl.nb, pl.gmax, p, grid, st, nullptr);
+    return dispatch(pl, p, grid, st, nullptr);
+}
+
+// Workspace of tqk_decode_q8_weights: the decode's tickets (always the whole region, so that the scores of
+// a call without splits do not touch the tickets of the calls it shares the workspace with) and partials,
+// then every q head's scores and final (max, sum).
+struct WeightScratch {
+    size_t ticket_bytes, part_off, score_off, ml_off, bytes;
+    long long score_stride;
+};
+
+WeightScratch weight_scratch(const tqk_decode_args *a, const Plan &pl) {
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    WeightScratch s{};
+    const size_t heads = (size_t)a->n_items * a->n_q_heads;
+    // whole 64-token tiles per row: the kernels store 16-token slices (a partial one's tail is -inf)
+    s.score_stride = ((long long)pl.max_len + DEC_T - 1) / DEC_T * DEC_T;
+    s.ticket_bytes = counters_region(a->n_items, pl.pairs);
+    s.part_off = s.ticket_bytes;
+    s.score_off = up(s.part_off + pl.part_bytes);
+    s.ml_off = up(s.score_off + heads * s.score_stride * sizeof(float));
+    s.bytes = s.ml_off + heads * sizeof(float2);
+    return s;
+}
+
+int check_weights(const tqk_decode_args *a, const tqk_weights_args *w) {
+    if (!a || !w) return fail(TQK_EINVAL, "tqk_decode_q8_weights: NULL args");
+    if (!w->weight || !w->weight_out) return fail(TQK_EINVAL, "tqk_decode_q8_weights: NULL weight or weight_out");
+    if (a->out_mode != TQK_OUT_NORMALIZED)
+        return fail(TQK_EINVAL, "tqk_decode_q8_weights: a weight needs the whole softmax, so only normalised output");
+    if ((reinterpret_cast<uintptr_t>(w->weight) | reinterpret_cast<uintptr_t>(w->weight_out) |
+         reinterpret_cast<uintptr_t>(w->position) | reinterpret_cast<uintptr_t>(w->new_pos)) & 3)
+        return fail(TQK_EALIGN, "tqk_decode_q8_weights: sums and positions must be 4-byte aligned");
+    if (w->position && !a->k_new)
+        return fail(TQK_EINVAL, "tqk_decode_q8_weights: position is written for appended rows (k_new, v_new)");
+    if (w->new_pos && !w->position) return fail(TQK_EINVAL, "tqk_decode_q8_weights: new_pos without position");
+    if (a->n_items > 1 && a->n_kv_heads > 0 && a->max_tokens > 0 &&
+        w->item_stride < (int64_t)a->n_kv_heads * a->max_tokens)
+        return fail(TQK_EINVAL, "tqk_decode_q8_weights: item_stride below n_kv_heads * max_tokens");
+    if (a->n_kv_heads > 65535) return fail(TQK_EINVAL, "tqk_decode_q8_weights: n_kv_heads > 65535");
+    return TQK_OK;
 }
 
 }  // namespace
 }  // namespace tqk
+
+extern "C" int tqk_decode_weights_workspace_size(const tqk_decode_args *a, size_t *bytes) {
+    Plan pl;
+    int rc = make_plan(a, &pl, false, true);
+    if (rc) return rc;
+    if (bytes) *bytes = weight_scratch(a, pl).bytes;
+    return TQK_OK;
+}
+
+extern "C" int tqk_decode_q8_weights(const tqk_decode_args *a, const tqk_weights_args *w, void *workspace,
+                                     size_t workspace_bytes, tqk_stream_t stream) {
+    int rc = check_weights(a, w);
+    if (rc) return rc;
+    Plan pl;
+    rc = make_plan(a, &pl, false, true);
+    if (rc) return rc;
+    rc = ensure_device();
+    if (rc) return rc;
+    const WeightScratch ws = weight_scratch(a, pl);
+    cudaStream_t st = (cudaStream_t)stream;
+    int *counters = nullptr;
+    uint8_t *base = nullptr;  // where ws's offsets from part_off on count from
+    if (!workspace) {
+        // library-owned: tickets in a buffer of their own, which scores and partials never touch
+        counters = library_counters(st, ws.ticket_bytes);
+        base = static_cast<uint8_t *>(library_workspace(st, ws.bytes - ws.ticket_bytes));
+        if (!counters || !base) return fail(TQK_ECUDA, "tqk_decode_q8_weights: cannot allocate the library workspace");
+    } else if (workspace_bytes < ws.bytes) {
+        return fail(TQK_EWORKSPACE, "tqk_decode_q8_weights: workspace smaller than tqk_decode_weights_workspace_size()");
+    } else if (reinterpret_cast<uintptr_t>(workspace) & 15) {
+        return fail(TQK_EALIGN, "tqk_decode_q8_weights: workspace must be 16-byte aligned");
+    } else {
+        counters = static_cast<int *>(workspace);
+        base = static_cast<uint8_t *>(workspace) + ws.ticket_bytes;
+    }
+    base -= ws.ticket_bytes;
+    DecodeParams p = fill_params(a, pl);
+    p.counters = counters;
+    p.part = reinterpret_cast<float *>(base + ws.part_off);
+    p.err = device_info()->err_word;
+    p.scores = reinterpret_cast<float *>(base + ws.score_off);
+    p.score_stride = ws.score_stride;
+    p.ml = reinterpret_cast<float2 *>(base + ws.ml_off);
+    p.len_cap = pl.max_len;
+    rc = pl.balanced ? dispatch(pl, p, dim3((unsigned)pl.bal_ctas), st, nullptr, true)
+                     : dispatch(pl, p, dim3((unsigned)pl.max_splits, (unsigned)pl.pairs, (unsigned)a->n_items), st, nullptr);
+    if (rc || pl.max_len == 0) return rc;  // nothing cached anywhere: no weights
+    WeightParams q{};
+    q.scores = p.scores;
+    q.score_stride = p.score_stride;
+    q.ml = p.ml;
+    q.group = p.group;
+    q.n_kv = p.n_kv;
+    q.max_tokens = p.max_tokens;
+    q.len_cap = p.len_cap;
+    q.lens = p.lens;
+    q.len0 = p.len0;
+    q.len_step = p.len_step;
+    q.weight = w->weight;
+    q.weight_out = w->weight_out;
+    q.item_stride = w->item_stride;
+    q.appended = a->k_new != nullptr;
+    q.position = w->position;
+    q.new_pos = w->new_pos;
+    q.new_pos0 = w->new_pos0;
+    const int per = WP_THREADS * WP_TOKENS;
+    const dim3 grid((unsigned)((pl.max_len + per - 1) / per), (unsigned)a->n_kv_heads, (unsigned)a->n_items);
+    return pl.mma ? launch_pdl(weight_sum_kernel<WT_LOG2>, grid, dim3(WP_THREADS), 0, st, q)
+                  : launch_pdl(weight_sum_kernel<WT_NAT>, grid, dim3(WP_THREADS), 0, st, q);
+}
 
 extern "C" int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t workspace_bytes,
                              tqk_stream_t stream) {
@@ -1301,9 +1461,7 @@ extern "C" int tqk_decode_q8_static(const tqk_decode_args *args, tqk_stream_t st
         e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess) return fail_cuda(e, "tqk_decode_q8_static: SM count");
         DecodeParams dummy{};
-        rc = pl.pack  ? dispatch_pack(pl.nb, dummy, dim3(1), nullptr, &occ)
-             : pl.mma ? dispatch_mma(pl.nb, pl.gmax, dummy, dim3(1), nullptr, &occ)
-                      : dispatch(pl.nb, pl.gmax, dummy, dim3(1), nullptr, &occ);
+        rc = dispatch(pl, dummy, dim3(1), nullptr, &occ);
         if (rc) return rc;
         const long long slots = (long long)sms * (occ > 0 ? occ : 1);
         const long long units = (long long)a.n_items * pl.pairs;
@@ -1337,8 +1495,7 @@ extern "C" int tqk_decode_q8_static(const tqk_decode_args *args, tqk_stream_t st
     p.part = pl.max_splits > 1 ? sc.part : nullptr;
     p.err = nullptr;  // no device error word: device-side checks still clamp or stop safely
     const dim3 grid((unsigned)pl.max_splits, (unsigned)pl.pairs, (unsigned)a.n_items);
-    if (pl.pack) return dispatch_pack(pl.nb, p, grid, st, nullptr);
-    return pl.mma ? dispatch_mma(pl.nb, pl.gmax, p, grid, st, nullptr) : dispatch(pl.nb, pl.gmax, p, grid, st, nullptr);
+    return dispatch(pl, p, grid, st, nullptr);
 }
 
 extern "C" int tqk_attend_q8(const tqk_block_q8 *k_plane, const tqk_block_q8 *v_plane, int n_q_heads,

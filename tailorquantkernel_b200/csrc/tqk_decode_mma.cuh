@@ -206,9 +206,11 @@ struct SliceState {
 // One 16-token slice (K rows at ks, V rows at vs, 144*NB/4-byte rows): scores,
 // online softmax (log2 domain), P*V into st.  FULL slices skip all masking;
 // partial ones mask tokens >= nvalid.  g = lane/4, t = lane%4.
-template <int NB, bool HI, bool FULL>
+//  WT: the lane's scores of row g (of rows g and g + 8 with HI) also go to srow (srow + 8 * sstride), those
+// of padding rows (row >= n_rows) to nowhere; a partial slice writes -inf for its missing tokens.
+template <int NB, bool HI, bool FULL, int WT>
 __device__ __forceinline__ void mma_slice(SliceState<NB, HI> &st, const uint8_t *ks, const uint8_t *vs, int nvalid,
-                                          float scale, int g, int t) {
+                                          float scale, int g, int t, float *srow, long long sstride, int n_rows) {
     constexpr int ROW = NB * BLOCK_BYTES;
     constexpr int NACC = SliceState<NB, HI>::NACC;
     const f32x2 scale2 = pk2(scale, scale);
@@ -242,6 +244,16 @@ __device__ __forceinline__ void mma_slice(SliceState<NB, HI> &st, const uint8_t 
             const int tk = nt * 8 + 2 * t;
             if (tk >= nvalid) sc[nt][0] = sc[nt][2] = -INFINITY;
             if (tk + 1 >= nvalid) sc[nt][1] = sc[nt][3] = -INFINITY;
+        }
+    }
+
+    if constexpr (WT != WT_NONE) {
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) {
+            float2 *d = reinterpret_cast<float2 *>(srow + nt * 8 + 2 * t);
+            if (g < n_rows) *d = make_float2(sc[nt][0], sc[nt][1]);
+            if (HI && g + 8 < n_rows)
+                *reinterpret_cast<float2 *>(srow + 8 * sstride + nt * 8 + 2 * t) = make_float2(sc[nt][2], sc[nt][3]);
         }
     }
 
@@ -361,7 +373,7 @@ __device__ __forceinline__ void mma_slice(SliceState<NB, HI> &st, const uint8_t 
     }
 }
 
-template <int NB, int GPAD>
+template <int NB, int GPAD, int WT>
 __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const DecodeParams p) {
     using L = MmaLayout<NB, GPAD>;
     constexpr int HD = L::HD, ROW = L::ROW, STAGES = L::STAGES;
@@ -381,11 +393,8 @@ __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const Decode
     const int slice = pair - kvh * p.head_slices;
     const int g0 = slice * p.heads_per_cta;
     const int G = min(p.heads_per_cta, p.group - g0);
-    int len = p.lens ? p.lens[item] : p.len0 + item * p.len_step;
-    if (len < 0 || len > p.max_tokens) {
-        if (tid == 0) record_error(p.err, DEVERR_BADLEN);
-        len = len < 0 ? 0 : p.max_tokens;
-    }
+    const int len = clamp_len(p, p.lens ? p.lens[item] : p.len0 + item * p.len_step,
+                              WT != WT_NONE ? p.len_cap : p.max_tokens, tid == 0);
     int n_splits = n_splits_of(len, p.split_tokens);
     if (n_splits > p.max_splits) {  // a device length above the max_len the grid was sized for
         if (tid == 0) record_error(p.err, DEVERR_BADLEN);
@@ -549,10 +558,11 @@ __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const Decode
                 }
                 __syncwarp();
             }
+            float *srow = WT != WT_NONE ? score_row_of(p, item, qh0 + g) + t0 + r0 : nullptr;
             if (nvalid >= 16)
-                mma_slice<NB, HI, true>(st, ks, vs, 16, p.scale, g, t);
+                mma_slice<NB, HI, true, WT>(st, ks, vs, 16, p.scale, g, t, srow, p.score_stride, G);
             else
-                mma_slice<NB, HI, false>(st, ks, vs, nvalid, p.scale, g, t);
+                mma_slice<NB, HI, false, WT>(st, ks, vs, nvalid, p.scale, g, t, srow, p.score_stride, G);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_release(&empty[slot]);
@@ -605,7 +615,8 @@ __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const Decode
             wsc[w * GPAD + tid] = e;
             Lsum += wl[w * GPAD + tid] * e;
         }
-        fm[tid] = M * 0.6931471805599453f;  // back to natural-log units for partials / merges
+        // back to natural-log units for partials / merges (WT_LOG2 merges in base 2)
+        fm[tid] = WT == WT_LOG2 ? M : M * 0.6931471805599453f;
         fl[tid] = Lsum;
     }
     cta_sync<1, MMA_WARPS * 32>();
@@ -615,8 +626,8 @@ __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const Decode
         for (int w = 0; w < MMA_WARPS; w++) a = fmaf(red[(w * GPAD + gg) * HD + c], wsc[w * GPAD + gg], a);
         return a;
     };
-    finish_split<HD, GPAD, MMA_WARPS * 32, 1>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, fm, fl, wts,
-                                              flag);
+    finish_split<HD, GPAD, MMA_WARPS * 32, 1, WT>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, fm, fl,
+                                                  wts, flag);
 }
 
 }  // namespace tqk

@@ -166,17 +166,23 @@ __device__ __forceinline__ void pack_scores(const uint32_t (&qa)[NB][2], const u
 // One warp step: tokens 0-15 of kv head A (k_a, v_a) and of kv head B (k_b,
 // v_b), 144*NB/4-byte rows; FULL steps skip the masking of tokens >= nvalid.
 // g = lane/4, t = lane%4, hb = g >= 4; mask_a / mask_b = f16x2 1.0 for the
-// lane's own head's k half of the PV operand, 0 for the other.
-template <int NB, bool FULL>
+// lane's own head's k half of the PV operand, 0 for the other.  WT: the lane's
+// four scores also go to srow[2t], [2t + 1], [8 + 2t], [9 + 2t] (-inf beyond
+// nvalid).
+template <int NB, bool FULL, int WT>
 __device__ __forceinline__ void pack_step(PackState<NB> &st, const uint8_t *k_a, const uint8_t *k_b,
                                           const uint8_t *v_a, const uint8_t *v_b, int nvalid, float scale, int g,
-                                          int t, bool hb, uint32_t mask_a, uint32_t mask_b) {
+                                          int t, bool hb, uint32_t mask_a, uint32_t mask_b, float *srow) {
     constexpr int ROW = NB * BLOCK_BYTES;
     const uint8_t *kmine = hb ? k_b : k_a;  // the lane's own head for scales
     const uint8_t *vmine = hb ? v_b : v_a;
 
     float s0, s1, s2, s3;
     pack_scores<NB, FULL>(st.qa, st.qb, st.qd2, k_a, k_b, kmine, nvalid, scale, g, t, s0, s1, s2, s3);
+    if constexpr (WT != WT_NONE) {
+        *reinterpret_cast<float2 *>(srow + 2 * t) = make_float2(s0, s1);
+        *reinterpret_cast<float2 *>(srow + 8 + 2 * t) = make_float2(s2, s3);
+    }
 
     // ---- online softmax of the row over its 16 tokens (the quad)
     float mx = fmaxf(fmaxf(s0, s1), fmaxf(s2, s3));
@@ -379,7 +385,7 @@ __device__ __forceinline__ void pack_patch(int pos, int t0, int r0, int lane, ui
 
 // Cross-warp reduction of a CTA's span: every consumer warp's unnormalised
 // P*V rows (red, [W][8][RED_STRIDE]) and its (m, l) go to shared memory; the
-// per-row maximum fm (natural log units), sum fl and per-warp weights wsc
+// per-row maximum fm (natural log units, log2 units with WT_LOG2), sum fl and per-warp weights wsc
 // follow.  acc(g, c) is then the CTA's sum for q row g, column c, relative to
 // fm[g].
 struct PackRed {
@@ -399,7 +405,7 @@ struct PackRed {
 };
 constexpr int PK_RED_SMALL = 3 * PK_WARPS * 8 + 16;  // floats of PackRed::small
 
-template <int NB, int RS>
+template <int NB, int RS, int WT>
 __device__ __forceinline__ void pack_reduce(const PackState<NB> &st, const PackRed &r, int warp, int g, int t,
                                             int tid) {
     float *wm = r.wm(), *wl = r.wl(), *wsc = r.wsc(), *fm = r.fm(), *fl = r.fl();
@@ -429,7 +435,7 @@ __device__ __forceinline__ void pack_reduce(const PackState<NB> &st, const PackR
             wsc[w * 8 + tid] = e;
             Lsum += wl[w * 8 + tid] * e;
         }
-        fm[tid] = M * 0.6931471805599453f;
+        fm[tid] = WT == WT_LOG2 ? M : M * 0.6931471805599453f;
         fl[tid] = Lsum;
     }
     cta_sync<1, PK_WARPS * 32>();
@@ -448,7 +454,7 @@ __device__ __forceinline__ void pack_reduce(const PackState<NB> &st, const PackR
 // timeout).  empty: this CTA holds no keys, or gave up on a wait.  Run by the
 // consumer threads only.
 constexpr uint64_t CL_WAIT_NS = 2000000000ull;  // above the 1 s bound of every wait before the merge
-template <int NB>
+template <int NB, int WT>
 __device__ __forceinline__ void pack_cluster_merge(const DecodeParams &p, uint8_t *smem, const PackRed &r, bool empty,
                                                    int tid, int item, int qh0, float *out_item) {
     using L = PackLayout<NB>;
@@ -502,12 +508,14 @@ __device__ __forceinline__ void pack_cluster_merge(const DecodeParams &p, uint8_
             float Ls = 0.0f;
             for (int rr = 0; rr < C; rr++) {
                 const float m = cm[rr * 8 + tid];
-                const float w = m == -INFINITY ? 0.0f : expf(m - M);
+                const float w = m == -INFINITY ? 0.0f : WT == WT_LOG2 ? exp2f(m - M) : expf(m - M);
                 cm[rr * 8 + tid] = w;
                 Ls += cl[rr * 8 + tid] * w;
             }
             fin[tid] = M;
             fin[8 + tid] = Ls;
+            if (WT != WT_NONE && rank == 0)
+                p.ml[(long long)item * (p.n_kv * p.group) + qh0 + tid] = make_float2(M, Ls);
         }
         cta_sync<1, NT>();
         for (int e = tid; e < n_share; e += NT) {
@@ -531,7 +539,7 @@ __device__ __forceinline__ void pack_cluster_merge(const DecodeParams &p, uint8_
     if (tid == 0) mbar_wait_cluster_bounded(&cbar[1], 0, CL_WAIT_NS, p.err);
 }
 
-template <int NB>
+template <int NB, int WT>
 __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel(const DecodeParams p) {
     using L = PackLayout<NB>;
     constexpr int HD = L::HD, ROW = L::ROW, STAGES = L::STAGES;
@@ -561,11 +569,8 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
     const int pair = blockIdx.y;  // kv heads 2*pair and 2*pair+1
     const int kvh_a = 2 * pair;
     const int G = 8;              // q heads served: 4 of each kv head
-    int len = p.lens ? p.lens[item] : p.len0 + item * p.len_step;
-    if (len < 0 || len > p.max_tokens) {
-        if (tid == 0) record_error(p.err, DEVERR_BADLEN);
-        len = len < 0 ? 0 : p.max_tokens;
-    }
+    const int len = clamp_len(p, p.lens ? p.lens[item] : p.len0 + item * p.len_step,
+                              WT != WT_NONE ? p.len_cap : p.max_tokens, tid == 0);
     int n_splits = n_splits_of(len, p.split_tokens);
     if (n_splits > p.max_splits) {  // a device length above the max_len the grid was sized for
         if (tid == 0) record_error(p.err, DEVERR_BADLEN);
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
         // partial); with len == 0 every CTA of the cluster (one item) leaves here or just below
         if (clustered && len > 0 && warp < PK_WARPS) {
             float *red = reinterpret_cast<float *>(smem);
-            pack_cluster_merge<NB>(p, smem, PackRed{red, red + L::RED_FLOATS}, true, tid, item, qh0, out_item);
+            pack_cluster_merge<NB, WT>(p, smem, PackRed{red, red + L::RED_FLOATS}, true, tid, item, qh0, out_item);
         }
         return;
     }
@@ -685,10 +690,11 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
             uint8_t *k_a = stg + r0 * ROW, *k_b = stg + L::PLANE + r0 * ROW;
             uint8_t *v_a = stg + 2 * L::PLANE + r0 * ROW, *v_b = stg + 3 * L::PLANE + r0 * ROW;
             if (do_append) pack_patch<NB>(pos, t0, r0, lane, k_a, k_b, v_a, v_b, newrow);
+            float *srow = WT != WT_NONE ? score_row_of(p, item, qh0 + g) + t0 + r0 : nullptr;
             if (nvalid >= PK_ROWS)
-                pack_step<NB, true>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b);
+                pack_step<NB, true, WT>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b, srow);
             else
-                pack_step<NB, false>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b);
+                pack_step<NB, false, WT>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b, srow);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_release(&empty[slot]);
@@ -700,19 +706,19 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
     float *red = reinterpret_cast<float *>(smem);  // [W][8][RED_STRIDE]
     PackRed r{red, red + L::RED_FLOATS};
     if (*timeout) {
-        if (clustered) pack_cluster_merge<NB>(p, smem, r, true, tid, item, qh0, out_item);
+        if (clustered) pack_cluster_merge<NB, WT>(p, smem, r, true, tid, item, qh0, out_item);
         return;
     }
 
-    pack_reduce<NB, L::RED_STRIDE>(st, r, warp, g, t, tid);
+    pack_reduce<NB, L::RED_STRIDE, WT>(st, r, warp, g, t, tid);
     if (clustered) {
-        pack_cluster_merge<NB>(p, smem, r, false, tid, item, qh0, out_item);
+        pack_cluster_merge<NB, WT>(p, smem, r, false, tid, item, qh0, out_item);
         return;
     }
     float *wts = r.fl() + 8;                       // [2][MAX_SPLITS][8]
     auto acc_of = [&](int gg, int c) { return r.acc<L::RED_STRIDE>(gg, c); };
-    finish_split<HD, 8, PK_WARPS * 32, 1>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, r.fm(), r.fl(),
-                                          wts, flag);
+    finish_split<HD, 8, PK_WARPS * 32, 1, WT>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, r.fm(),
+                                              r.fl(), wts, flag);
 }
 
 
@@ -783,7 +789,7 @@ __device__ __forceinline__ BalSeg bal_segment(const int *pre, const int *lens, i
     return s;
 }
 
-template <int NB>
+template <int NB, int WT>
 __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_kernel(const DecodeParams p) {
     using L = PackBalLayout<NB>;
     constexpr int HD = L::HD, ROW = L::ROW, STAGES = L::STAGES;
@@ -813,11 +819,8 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
             const int i = lane * PER + k;
             int len = 0;
             if (i < n_items) {
-                len = p.lens ? p.lens[i] : p.len0 + i * p.len_step;
-                if (len < 0 || len > p.max_tokens) {
-                    record_error(p.err, DEVERR_BADLEN);
-                    len = len < 0 ? 0 : p.max_tokens;
-                }
+                len = clamp_len(p, p.lens ? p.lens[i] : p.len0 + i * p.len_step,
+                                WT != WT_NONE ? p.len_cap : p.max_tokens, true);
                 lens[i] = len;
             }
             tl[k] = (len + PK_T - 1) / PK_T * pairs;
@@ -952,10 +955,14 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
                     uint8_t *k_a = stg + r0 * ROW, *k_b = stg + L::PLANE + r0 * ROW;
                     uint8_t *v_a = stg + 2 * L::PLANE + r0 * ROW, *v_b = stg + 3 * L::PLANE + r0 * ROW;
                     if (do_append) pack_patch<NB>(pos, t0, r0, lane, k_a, k_b, v_a, v_b, newrow);
+                    float *srow =
+                        WT != WT_NONE ? score_row_of(p, sg.item, 2 * sg.pair * p.group + g) + t0 + r0 : nullptr;
                     if (nvalid >= PK_ROWS)
-                        pack_step<NB, true>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b);
+                        pack_step<NB, true, WT>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b,
+                                                srow);
                     else
-                        pack_step<NB, false>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b);
+                        pack_step<NB, false, WT>(st, k_a, k_b, v_a, v_b, nvalid, p.scale, g, t, hb, mask_a, mask_b,
+                                                 srow);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive_release(&empty[slot]);
@@ -965,7 +972,7 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
         cta_sync<1, PK_WARPS * 32>();
         if (*timeout) return;
 
-        pack_reduce<NB, L::RED_STRIDE>(st, red, warp, g, t, tid);
+        pack_reduce<NB, L::RED_STRIDE, WT>(st, red, warp, g, t, tid);
         const int Tn = pre[n_items];
         const int Cn = min((int)gridDim.x, Tn);
         const int cn = blockIdx.x;
@@ -979,7 +986,7 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
         int *tickets = p.counters + unit * p.tickets_per_unit;
         float *out_item = p.out + (long long)sg.item * p.out_item_stride;
         auto acc_of = [&](int gg, int cc) { return red.acc<L::RED_STRIDE>(gg, cc); };
-        finish_split_at<HD, G, PK_WARPS * 32, 1>(p, tid, pb, tickets, cn - c0, c1 - c0 + 1, sg.item,
+        finish_split_at<HD, G, PK_WARPS * 32, 1, WT>(p, tid, pb, tickets, cn - c0, c1 - c0 + 1, sg.item,
                                                  2 * sg.pair * p.group, G,
                                                  out_item, acc_of, red.fm(), red.fl(), red.red, flag);
         gt = sg.ubase + sg.lt1;

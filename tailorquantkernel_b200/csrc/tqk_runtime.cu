@@ -133,7 +133,7 @@ extern "C" const char *tqk_status_string(int status) {
         case TQK_ENODEV: return "no CUDA device";
         case TQK_ETIMEOUT: return "device wait timed out";
         case TQK_EUNSUPPORTED: return "unsupported shape";
-        case TQK_EDEVLEN: return "a device-side length was outside [0, max_tokens] and was clamped";
+        case TQK_EDEVLEN: return "a device-side length, offset or index was out of range and was clamped";
         default: return "unknown status";
     }
 }

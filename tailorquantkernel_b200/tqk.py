@@ -93,6 +93,53 @@ tqk_decode_workspace_size = _sig("tqk_decode_workspace_size", [ctypes.POINTER(De
 tqk_workspace_init = _sig("tqk_workspace_init", [_vp, _sz, _vp])
 tqk_decode_q8 = _sig("tqk_decode_q8", [ctypes.POINTER(DecodeArgs), _vp, _sz, _vp])
 tqk_decode_q8_static = _sig("tqk_decode_q8_static", [ctypes.POINTER(DecodeArgs), _vp])
+
+
+class WeightsArgs(ctypes.Structure):
+    """Mirror of tqk_weights_args (include/tqk.h)."""
+    _fields_ = [("weight", _vp), ("weight_out", _vp), ("item_stride", _i64), ("position", _vp), ("new_pos", _vp),
+                ("new_pos0", _i)]
+
+
+class EvictArgs(ctypes.Structure):
+    """Mirror of tqk_evict_args (include/tqk.h)."""
+    _fields_ = [
+        ("k", _vp), ("v", _vp),
+        ("item_stride", _i64),
+        ("n_items", _i), ("n_kv_heads", _i), ("head_dim", _i), ("max_tokens", _i),
+        ("lens", _vp),
+        ("len0", _i), ("len_step", _i),
+        ("max_len", _i),
+        ("budget", _i),
+        ("n_first", _i), ("n_recent", _i),
+        ("weight", _vp), ("weight_out", _vp),
+        ("position", _vp), ("position_out", _vp),
+        ("stat_item_stride", _i64),
+        ("lens_out", _vp),
+    ]
+
+
+class LogitsArgs(ctypes.Structure):
+    """Mirror of tqk_logits_args (include/tqk.h)."""
+    _fields_ = [
+        ("logits", _vp), ("logits_stride", _i64),
+        ("out", _vp), ("out_stride", _i64),
+        ("choice", _vp),
+        ("n_rows", _i), ("vocab_size", _i),
+        ("tokens", _vp), ("token_offsets", _vp), ("n_tokens", _i),
+        ("prompt_lens", _vp),
+        ("repetition", _vp), ("frequency", _vp), ("presence", _vp),
+        ("bias_tokens", _vp), ("bias_values", _vp), ("bias_offsets", _vp), ("n_bias", _i),
+        ("mask", _vp), ("mask_stride", _i64), ("mask_rows", _vp), ("n_mask_rows", _i),
+    ]
+
+
+tqk_decode_weights_workspace_size = _sig("tqk_decode_weights_workspace_size",
+                                         [ctypes.POINTER(DecodeArgs), ctypes.POINTER(_sz)])
+tqk_decode_q8_weights = _sig("tqk_decode_q8_weights",
+                             [ctypes.POINTER(DecodeArgs), ctypes.POINTER(WeightsArgs), _vp, _sz, _vp])
+tqk_evict_q8 = _sig("tqk_evict_q8", [ctypes.POINTER(EvictArgs), _vp])
+tqk_process_logits = _sig("tqk_process_logits", [ctypes.POINTER(LogitsArgs), _vp])
 tqk_qk_norm_rope = _sig("tqk_qk_norm_rope", [_vp, _vp, _i, _i64, _i64, _i, _i, _i, _vp, _vp, _i64, _f, _vp, _vp,
                                               _i64, _vp])
 tqk_packed_matrix_bytes = _sig("tqk_packed_matrix_bytes", [_i, _i, ctypes.c_char], _sz)
@@ -197,6 +244,7 @@ EXPORTED = [
     "tqk_decode_q8_gather", "tqk_decode_unit_count", "tqk_gather_collect",
     "tqk_forward_scratch_bytes", "tqk_forward_token",
     "tqk_fill_normal", "tqk_fill_uniform", "tqk_xorshift_jump",
+    "tqk_decode_weights_workspace_size", "tqk_decode_q8_weights", "tqk_evict_q8", "tqk_process_logits",
 ]
 
 
@@ -225,6 +273,13 @@ def _ptr(t) -> Optional[int]:
     if not t.is_contiguous():
         raise ValueError("tensor must be contiguous")
     return t.data_ptr()
+
+
+def _typed(t, dtype: str) -> Optional[int]:
+    """_ptr of a tensor that must have the named torch dtype (addresses are taken as they are)."""
+    if t is not None and not isinstance(t, int) and str(t.dtype) != f"torch.{dtype}":
+        raise ValueError(f"expected a {dtype} tensor, got {t.dtype}")
+    return _ptr(t)
 
 
 def _stream(stream) -> int:
@@ -324,6 +379,96 @@ def decode(args: DecodeArgs, workspace=None, stream=None) -> None:
     ws = _ptr(workspace) if workspace is not None else None
     nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     check(tqk_decode_q8(ctypes.byref(args), ws, nbytes, _stream(stream)), "tqk_decode_q8")
+
+
+def weights_args(weight, weight_out=None, *, item_stride=0, position=None, new_pos=None, new_pos0=0) -> WeightsArgs:
+    """tqk_weights_args: running sums [..., n_kv, max_tokens] (fp32) and their positions (int32).  weight_out None
+    adds in place."""
+    w = WeightsArgs()
+    w.weight = _typed(weight, "float32")
+    w.weight_out = w.weight if weight_out is None else _typed(weight_out, "float32")
+    w.item_stride = item_stride
+    w.position, w.new_pos, w.new_pos0 = _typed(position, "int32"), _typed(new_pos, "int32"), new_pos0
+    return w
+
+
+def decode_weights(args: DecodeArgs, weights: WeightsArgs, workspace=None, stream=None) -> None:
+    """tqk_decode_q8_weights: the decode, and each cached row's attention weight added to its running sum."""
+    ws = _ptr(workspace) if workspace is not None else None
+    nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    check(tqk_decode_q8_weights(ctypes.byref(args), ctypes.byref(weights), ws, nbytes, _stream(stream)),
+          "tqk_decode_q8_weights")
+
+
+def decode_weights_workspace_size(args: DecodeArgs) -> int:
+    out = _sz(0)
+    check(tqk_decode_weights_workspace_size(ctypes.byref(args), ctypes.byref(out)),
+          "tqk_decode_weights_workspace_size")
+    return out.value
+
+
+def evict_args(k, v, n_kv, head_dim, max_tokens, budget, *, weight, weight_out=None, position=None, position_out=None,
+               n_items=1, item_stride_blocks=0, stat_item_stride=0, lens=None, len0=0, len_step=0, max_len=0, n_first=0,
+               n_recent=0, lens_out=None) -> EvictArgs:
+    """tqk_evict_args.  weight_out / position_out None: in place."""
+    a = EvictArgs()
+    a.k, a.v, a.item_stride = _ptr(k), _ptr(v), item_stride_blocks
+    a.n_items, a.n_kv_heads, a.head_dim, a.max_tokens = n_items, n_kv, head_dim, max_tokens
+    a.lens = _typed(lens, "int32")
+    a.len0, a.len_step, a.max_len = len0, len_step, max_len
+    a.budget, a.n_first, a.n_recent = budget, n_first, n_recent
+    a.weight = _typed(weight, "float32")
+    a.weight_out = a.weight if weight_out is None else _typed(weight_out, "float32")
+    a.position = _typed(position, "int32")
+    a.position_out = a.position if position_out is None else _typed(position_out, "int32")
+    a.stat_item_stride = stat_item_stride
+    a.lens_out = _typed(lens_out, "int32")
+    return a
+
+
+def evict(args: EvictArgs, stream=None) -> None:
+    """tqk_evict_q8: every (item, kv head) goes down to its budget of rows."""
+    check(tqk_evict_q8(ctypes.byref(args), _stream(stream)), "tqk_evict_q8")
+
+
+def _row_ptr(t, dtype: str):
+    """Address, row stride, rows and columns of a CUDA matrix whose rows are contiguous."""
+    if str(t.dtype) != f"torch.{dtype}":
+        raise ValueError(f"expected a {dtype} tensor, got {t.dtype}")
+    if not t.is_cuda or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("expected a CUDA matrix with contiguous rows")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1], t.shape[0], t.shape[1]
+
+
+def logits_args(logits, *, out=None, choice=None, tokens=None, token_offsets=None, n_tokens=None, prompt_lens=None,
+                repetition=None, frequency=None, presence=None, bias_tokens=None, bias_values=None, bias_offsets=None,
+                n_bias=None, mask=None, mask_rows=None) -> LogitsArgs:
+    """tqk_logits_args from logits [n_rows, vocab] (rows may be strided), out likewise (None: only the choice),
+    packed histories and bias lists with their offsets [n_rows + 1], and mask words [n_mask_rows, words] (int32)."""
+    a = LogitsArgs()
+    a.logits, a.logits_stride, a.n_rows, a.vocab_size = _row_ptr(logits, "float32")
+    if out is not None:
+        a.out, a.out_stride, rows, cols = _row_ptr(out, "float32")
+        if (rows, cols) != (a.n_rows, a.vocab_size):
+            raise ValueError("out must have the shape of logits")
+    a.choice = _typed(choice, "int32")
+    a.tokens, a.token_offsets, a.prompt_lens = (_typed(t, "int32") for t in (tokens, token_offsets, prompt_lens))
+    a.n_tokens = n_tokens if n_tokens is not None else tokens.numel() if tokens is not None else 0
+    a.repetition, a.frequency, a.presence = (_typed(t, "float32") for t in (repetition, frequency, presence))
+    a.bias_tokens, a.bias_values = _typed(bias_tokens, "int32"), _typed(bias_values, "float32")
+    a.bias_offsets = _typed(bias_offsets, "int32")
+    a.n_bias = n_bias if n_bias is not None else bias_tokens.numel() if bias_tokens is not None else 0
+    if mask is not None:
+        a.mask, a.mask_stride, a.n_mask_rows, words = _row_ptr(mask, "int32")
+        if words < (a.vocab_size + 31) // 32:
+            raise ValueError("mask rows need a bit per token")
+    a.mask_rows = _typed(mask_rows, "int32")
+    return a
+
+
+def process_logits(args: LogitsArgs, stream=None) -> None:
+    """tqk_process_logits: penalties, biases and masks on the next token's logits, and the greedy choice."""
+    check(tqk_process_logits(ctypes.byref(args), _stream(stream)), "tqk_process_logits")
 
 
 def qk_norm_rope(q, k, n_items, n_q, n_kv, head_dim, q_norm=None, k_norm=None, eps=1e-6, rope_cos=None,

@@ -1,0 +1,161 @@
+"""Refusals of tqk_decode_q8_weights, tqk_evict_q8 and tqk_process_logits, which all come before any device work, the
+argument structs' layouts, and the plain implementations' own checks -- without a GPU."""
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from _cache_ops import attend64, evict_ref, logits_ref, pack_bits, weight_bound
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+FAKE = 4096  # an aligned address that nothing touches
+
+
+@pytest.fixture(scope="module")
+def tqk():
+    from tailorquantkernel_b200 import tqk as t
+    return t
+
+
+@pytest.mark.parametrize("struct,c_name", [("WeightsArgs", "tqk_weights_args"), ("EvictArgs", "tqk_evict_args"),
+                                           ("LogitsArgs", "tqk_logits_args")])
+def test_struct_layouts_match_c(tqk, tmp_path, struct, c_name):
+    cls = getattr(tqk, struct)
+    fields = [f for f, _ in cls._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "tqk.h"\nint main(void){\n'
+                   f'printf("%zu\\n", sizeof({c_name}));\n' +
+                   "".join(f'printf("%zu\\n", offsetof({c_name}, {f}));\n' for f in fields) + "return 0;}\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["/usr/bin/gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    vals = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert vals == [ctypes.sizeof(cls)] + [getattr(cls, f).offset for f in fields]
+
+
+def _fill(struct, good, change):
+    for k, v in {**good, **change}.items():
+        setattr(struct, k, v)
+    return struct
+
+
+DECODE = dict(k=FAKE, v=FAKE, q=FAKE, out=FAKE, n_items=2, n_q_heads=8, n_kv_heads=2, head_dim=128, max_tokens=64,
+              item_stride=2 * 64 * 4, len0=10)
+WEIGHTS = dict(weight=FAKE, weight_out=FAKE, item_stride=2 * 64)
+
+
+@pytest.mark.parametrize("decode,weights,status", [
+    ({}, dict(weight=None), "EINVAL"), ({}, dict(weight_out=None), "EINVAL"),
+    ({}, dict(weight=FAKE + 2), "EALIGN"), ({}, dict(weight_out=FAKE + 1), "EALIGN"),
+    (dict(out_mode=1), {}, "EINVAL"),                      # partial output has no weights yet
+    ({}, dict(item_stride=127), "EINVAL"), ({}, dict(item_stride=0), "EINVAL"),
+    ({}, dict(position=FAKE), "EINVAL"),                   # positions belong to appended rows
+    (dict(k_new=FAKE, v_new=FAKE), dict(new_pos=FAKE), "EINVAL"),
+    (dict(k_new=FAKE), {}, "EINVAL"), (dict(n_q_heads=7), {}, "EINVAL"), (dict(head_dim=96), {}, "EUNSUPPORTED"),
+    (dict(k=FAKE + 8), {}, "EALIGN"), (dict(len0=65), {}, "EPOS"), (dict(len0=0, k_new=FAKE, v_new=FAKE), {}, "EPOS"),
+    (dict(lens=FAKE, max_len=65), {}, "EINVAL"), (dict(q_norm=FAKE), {}, "EINVAL"), (dict(rope_cos=FAKE), {}, "EINVAL"),
+    (dict(n_items=0), {}, "EINVAL"), (dict(q=None), {}, "EINVAL"),
+])
+def test_decode_weights_refusals(tqk, decode, weights, status):
+    a, w = _fill(tqk.DecodeArgs(), DECODE, decode), _fill(tqk.WeightsArgs(), WEIGHTS, weights)
+    assert tqk.tqk_decode_q8_weights(ctypes.byref(a), ctypes.byref(w), None, 0, None) == getattr(tqk, status)
+    assert tqk.tqk_last_error()
+
+
+def test_null_structs(tqk):
+    a, w = tqk.DecodeArgs(), tqk.WeightsArgs()
+    assert tqk.tqk_decode_q8_weights(None, ctypes.byref(w), None, 0, None) == tqk.EINVAL
+    assert tqk.tqk_decode_q8_weights(ctypes.byref(a), None, None, 0, None) == tqk.EINVAL
+    assert tqk.tqk_decode_weights_workspace_size(None, None) == tqk.EINVAL
+    assert tqk.tqk_evict_q8(None, None) == tqk.EINVAL
+    assert tqk.tqk_process_logits(None, None) == tqk.EINVAL
+
+
+EVICT = dict(k=FAKE, v=FAKE, weight=FAKE, weight_out=FAKE, position=FAKE, position_out=FAKE, n_items=2, n_kv_heads=2,
+             head_dim=128, max_tokens=64, item_stride=2 * 64 * 4, stat_item_stride=2 * 64, len0=60, budget=32, n_first=4,
+             n_recent=8)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(k=None), "EINVAL"), (dict(weight_out=None), "EINVAL"), (dict(position_out=None), "EINVAL"),
+    (dict(position=None, position_out=None), "EINVAL"),    # protected positions need positions
+    (dict(n_items=0), "EINVAL"), (dict(head_dim=48), "EINVAL"), (dict(head_dim=160), "EUNSUPPORTED"),
+    (dict(budget=0), "EINVAL"), (dict(budget=65), "EINVAL"), (dict(n_first=25), "EINVAL"), (dict(n_first=-1), "EINVAL"),
+    (dict(n_recent=2 ** 31 - 1), "EINVAL"), (dict(item_stride=511), "EINVAL"), (dict(stat_item_stride=127), "EINVAL"),
+    (dict(len0=65), "EPOS"), (dict(len0=-1), "EPOS"), (dict(len_step=5), "EPOS"), (dict(lens=FAKE, max_len=65), "EINVAL"),
+    (dict(lens=FAKE, max_len=-1), "EINVAL"), (dict(k=FAKE + 4), "EALIGN"), (dict(item_stride=513), "EALIGN"),
+    (dict(head_dim=64, k=FAKE + 2), "EALIGN"), (dict(weight=FAKE + 2), "EALIGN"), (dict(position_out=FAKE + 1), "EALIGN"),
+    (dict(n_items=1, max_tokens=600000, len0=520000), "EUNSUPPORTED"),
+    (dict(n_items=70000), "EINVAL"),
+])
+def test_evict_refusals(tqk, change, status):
+    assert tqk.tqk_evict_q8(ctypes.byref(_fill(tqk.EvictArgs(), EVICT, change)), None) == getattr(tqk, status)
+    assert tqk.tqk_last_error()
+
+
+LOGITS = dict(logits=FAKE, out=FAKE * 2, choice=FAKE, n_rows=2, vocab_size=100, tokens=FAKE, token_offsets=FAKE, n_tokens=5,
+              repetition=FAKE, bias_tokens=FAKE, bias_values=FAKE, bias_offsets=FAKE, n_bias=3, mask=FAKE, n_mask_rows=2)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(logits=None), "EINVAL"), (dict(out=None, choice=None), "EINVAL"), (dict(n_rows=0), "EINVAL"),
+    (dict(vocab_size=0), "EINVAL"), (dict(n_rows=70000, n_mask_rows=70000), "EINVAL"),
+    (dict(vocab_size=2 ** 30), "EUNSUPPORTED"), (dict(n_tokens=2 ** 30), "EUNSUPPORTED"),
+    (dict(logits_stride=99), "EINVAL"), (dict(out_stride=99), "EINVAL"), (dict(out=FAKE, out_stride=101), "EINVAL"),
+    (dict(tokens=None), "EINVAL"), (dict(token_offsets=None), "EINVAL"), (dict(n_tokens=-1), "EINVAL"),
+    (dict(bias_values=None), "EINVAL"), (dict(bias_offsets=None), "EINVAL"), (dict(bias_tokens=None), "EINVAL"),
+    (dict(n_bias=-1), "EINVAL"), (dict(mask_stride=3), "EINVAL"), (dict(n_mask_rows=1), "EINVAL"),
+    (dict(mask=None, mask_rows=FAKE), "EINVAL"), (dict(logits=FAKE + 2), "EALIGN"), (dict(mask=FAKE + 1), "EALIGN"),
+])
+def test_logits_refusals(tqk, change, status):
+    assert tqk.tqk_process_logits(ctypes.byref(_fill(tqk.LogitsArgs(), LOGITS, change)), None) == getattr(tqk, status)
+    assert tqk.tqk_last_error()
+
+
+def test_python_helpers_refuse_wrong_types(tqk):
+    """Index arrays of another type than int32, or sums of another than fp32, would be misread: refused by name."""
+    import torch
+    f, i = torch.zeros(4), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="CUDA"):
+        tqk.weights_args(f)
+    with pytest.raises(ValueError, match="CUDA"):
+        tqk.logits_args(torch.zeros(2, 3))
+    with pytest.raises(ValueError, match="int32"):
+        tqk.weights_args(FAKE, position=i)
+    with pytest.raises(ValueError, match="float32"):
+        tqk.weights_args(f.double())
+    with pytest.raises(ValueError, match="int32"):
+        tqk.evict_args(FAKE, FAKE, 1, 32, 4, 2, weight=FAKE, lens=i)
+    with pytest.raises(ValueError, match="float32"):
+        tqk.logits_args(torch.zeros(2, 3, dtype=torch.bfloat16))
+
+
+def test_plain_eviction():
+    """The plain implementation on a case worked out by hand."""
+    w = np.array([5, 1, 4, np.nan, 3, 3, 0.5, 9], np.float32)
+    p = np.arange(8, dtype=np.int32)
+    keep, dst, src = evict_ref(w, p, 8, 4, 1, 2)       # protected: 0, 6, 7; then the largest of the rest: 2
+    assert np.flatnonzero(keep).tolist() == [0, 2, 6, 7] and dst.tolist() == [1, 3] and src.tolist() == [6, 7]
+    keep, dst, src = evict_ref(w, None, 8, 5, 0, 0)    # 9, 5, 4, then the lower of the two threes
+    assert np.flatnonzero(keep).tolist() == [0, 2, 4, 5, 7] and dst.tolist() == [1, 3] and src.tolist() == [5, 7]
+    keep, dst, src = evict_ref(w, None, 8, 4, 0, 0)
+    assert np.flatnonzero(keep).tolist() == [0, 2, 4, 7] and dst.tolist() == [1, 3] and src.tolist() == [4, 7]
+
+
+def test_plain_logits():
+    x = np.array([2, -2, 0, 1, 5], np.float32)
+    y, best = logits_ref(x, tokens=np.array([0, 1, 1, 9, -1], np.int32), prompt=1, repetition=2.0, frequency=0.5,
+                         presence=0.25, bias=[(3, 1.0), (3, 2.0), (7, 100.0)], allowed=np.array([1, 1, 1, 1, 0], bool))
+    assert y.tolist() == [1.0, -4.0 - 1.0 - 0.25, 0.0, 4.0, -np.inf] and best == 3
+    assert logits_ref(x, allowed=np.zeros(5, bool))[1] == -1
+    assert pack_bits(np.array([[0] * 31 + [1, 1]], bool)).view(np.uint32).tolist() == [[2 ** 31, 1]]
+
+
+def test_plain_attention_sums_to_one_per_head():
+    import oracle
+    rng = np.random.default_rng(0)
+    port = oracle.Oracle("port")
+    q, k, v = (port.quantize_rows(rng.standard_normal(s, dtype=np.float32)) for s in ((2, 6, 64), (2, 2, 9, 64), (2, 2, 9, 64)))
+    _, w, big = attend64(q, k, v, [9, 4])
+    assert np.allclose(w.sum(-1), 3.0) and (w[1, :, 4:] == 0).all() and 0 < weight_bound(2, big, 9) < 1e-5

@@ -1,0 +1,192 @@
+"""tqk_process_logits against a plain implementation that rounds every step to fp32 as the operator defines it: the
+outputs are compared bit for bit (NaN with NaN)."""
+import numpy as np
+import pytest
+
+from _cache_ops import logits_ref, pack_bits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def tqk(cuda):
+    from tailorquantkernel_b200 import tqk as t
+    return t
+
+
+def _packed(rng, rows, lo, hi, vocab, wild):
+    """Packed lists of token ids with their offsets; `wild` adds ids outside the vocabulary."""
+    lens = rng.integers(lo, hi + 1, rows)
+    lens[0], lens[-1] = hi, lo
+    off = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    ids = (rng.random(off[-1]) ** 3 * vocab).astype(np.int32)  # repeats many
+    if wild and ids.size:
+        ids[::7] = rng.choice([-1, vocab, vocab + 5, -2 ** 31, 2 ** 31 - 1], ids[::7].shape)
+    return ids, off
+
+
+CASES = [  # rows, vocab, history, biases, allowed share, penalties (repetition, frequency, presence), row padding
+    (1, 1, (3, 3), (2, 2), 1.0, (1, 1, 1), 0),
+    (2, 31, (0, 40), (0, 9), 0.5, (1, 1, 1), 1),
+    (3, 33, (0, 5), None, 0.1, (1, 0, 0), 31),
+    (1, 127, (500, 500), (64, 64), None, (0, 1, 0), 0),
+    (5, 128, (0, 300), (0, 30), 0.5, (0, 0, 1), 4),
+    (4, 2048, None, (0, 7), 0.3, None, 0),
+    (4, 2050, (1, 2000), None, None, (1, 1, 1), 2),       # rows of 8-byte alignment
+    (7, 32003, (0, 2049), (0, 11), 0.02, (1, 1, 1), 0),   # odd rows
+    (3, 131072, (0, 9000), (5, 50), 0.9, (1, 1, 1), 0),   # a whole piece per CTA
+    (2, 131077, (100, 100), (3, 3), 0.9, (1, 1, 1), 3),   # and some more
+    (2, 300001, (0, 5000), (0, 40), 0.5, (1, 1, 1), 7),   # several pieces, unaligned
+    (2, 299008, (0, 5000), (0, 40), 0.5, (1, 1, 1), 0),   # several pieces, aligned
+    (3, 50257, None, None, 0.5, None, 0),
+    (3, 50256, None, None, None, None, 0),
+]
+
+
+@pytest.mark.parametrize("mode", ["out", "in place", "choice"])
+@pytest.mark.parametrize("rows,vocab,history,biases,share,penal,pad", CASES)
+def test_against_the_definition(tqk, cuda, rows, vocab, history, biases, share, penal, pad, mode):
+    import torch
+    rng = np.random.default_rng(vocab + rows)
+    x = rng.standard_normal((rows, vocab), dtype=np.float32) * 3
+    special = np.array([np.inf, -np.inf, np.nan, 0.0, -0.0, 1e-40, 3e38], np.float32)
+    if vocab > 30 and share is not None:  # odd values, also in masked places
+        at = rng.integers(0, vocab, 40)
+        x[:, at] = special[rng.integers(0, len(special) - (rows == 1), (rows, 40))]
+    kw, want_kw = {}, [dict() for _ in range(rows)]
+
+    def dev(a):
+        return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+    if history:
+        ids, off = _packed(rng, rows, *history, vocab, wild=vocab > 1)
+        prompts = rng.integers(-1, history[1] + 2, rows).astype(np.int32)  # some beyond the history
+        kw.update(tokens=dev(ids) if ids.size else dev(np.zeros(1, np.int32)), n_tokens=ids.size, token_offsets=dev(off),
+                  prompt_lens=dev(prompts))
+        for name, on in zip(("repetition", "frequency", "presence"), penal):
+            if on:
+                val = (rng.random(rows, dtype=np.float32) + (0.7 if name == "repetition" else -0.3))
+                kw[name] = dev(val)
+                for r in range(rows):
+                    want_kw[r][name] = val[r]
+        for r in range(rows):
+            want_kw[r].update(tokens=ids[off[r]:off[r + 1]], prompt=int(prompts[r]))
+    if biases:
+        ids, off = _packed(rng, rows, *biases, min(vocab, 50), wild=vocab > 1)  # repeated tokens
+        val = rng.standard_normal(ids.size, dtype=np.float32) * 5
+        kw.update(bias_tokens=dev(ids) if ids.size else dev(np.zeros(1, np.int32)),
+                  bias_values=dev(val) if ids.size else dev(np.zeros(1, np.float32)), n_bias=ids.size, bias_offsets=dev(off))
+        for r in range(rows):
+            want_kw[r]["bias"] = list(zip(ids[off[r]:off[r + 1]].tolist(), val[off[r]:off[r + 1]]))
+    if share is not None:
+        allowed = rng.random((rows, vocab)) < share
+        if rows > 2:
+            allowed[1] = False  # a grammar that leaves nothing
+        kw["mask"] = dev(pack_bits(allowed))
+        for r in range(rows):
+            want_kw[r]["allowed"] = allowed[r]
+    buf = torch.full((rows, vocab + pad), 7.0, device="cuda")
+    logits = buf[:, :vocab]
+    logits.copy_(torch.from_numpy(x))
+    obuf = buf if mode == "in place" else torch.full((rows, vocab + pad), 7.0, device="cuda")
+    choice = torch.full((rows,), -9, dtype=torch.int32, device="cuda")
+    tqk.process_logits(tqk.logits_args(logits, out=None if mode == "choice" else obuf[:, :vocab], choice=choice, **kw))
+    torch.cuda.synchronize()
+    got = obuf.cpu().numpy()
+    assert (got[:, vocab:] == 7.0).all()
+    for r in range(rows):
+        ref, best = logits_ref(x[r], **want_kw[r])
+        if mode == "choice":
+            assert (got[r] == 7.0).all()
+        else:
+            nan = np.isnan(ref)
+            assert np.array_equal(np.isnan(got[r, :vocab]), nan)
+            assert np.array_equal(got[r, :vocab][~nan].view(np.uint32), ref[~nan].view(np.uint32))
+        assert choice[r].item() == best
+    if mode != "in place":
+        assert np.array_equal(logits.cpu().numpy().view(np.uint32), x.view(np.uint32))
+    assert tqk.device_status() == 0
+
+
+def test_ties_go_to_the_lowest_token(tqk, cuda):
+    import torch
+    for vocab in (100, 40000, 140001):
+        x = torch.zeros((3, vocab), device="cuda")
+        x[0, [5, vocab // 2, vocab - 1]] = 2.0
+        x[1, vocab - 1] = 2.0
+        choice = torch.empty(3, dtype=torch.int32, device="cuda")
+        tqk.process_logits(tqk.logits_args(x, choice=choice))
+        assert choice.tolist() == [5, vocab - 1, 0]
+
+
+def test_mask_rows(tqk, cuda):
+    """Rows share mask rows, go without one (-1), and an index out of range allows nothing and is reported."""
+    import torch
+    vocab = 5000
+    rng = np.random.default_rng(1)
+    x = torch.from_numpy(rng.standard_normal((5, vocab), dtype=np.float32)).cuda()
+    allowed = rng.random((2, vocab)) < 0.5
+    out, choice = torch.empty_like(x), torch.empty(5, dtype=torch.int32, device="cuda")
+    mask = torch.from_numpy(pack_bits(allowed)).cuda()
+    rows = torch.tensor([1, -1, 0, 1, -1], dtype=torch.int32, device="cuda")
+    tqk.process_logits(tqk.logits_args(x, out=out, choice=choice, mask=mask, mask_rows=rows))
+    for r, m in enumerate(rows.tolist()):
+        ref, best = logits_ref(x[r].cpu().numpy(), allowed=allowed[m] if m >= 0 else None)
+        assert np.array_equal(out[r].cpu().numpy(), ref) and choice[r].item() == best
+    assert tqk.device_status() == 0
+    for bad in (2, -2):
+        rows[3] = bad
+        tqk.process_logits(tqk.logits_args(x, out=out, choice=choice, mask=mask, mask_rows=rows))
+        assert choice[3].item() == -1 and torch.isinf(out[3]).all() and choice[1].item() == int(x[1].argmax())
+        assert tqk.tqk_device_error_status(tqk.device_status(clear=True)) == tqk.EDEVLEN
+
+
+def test_bad_offsets_are_clamped_and_reported(tqk, cuda):
+    import torch
+    vocab = 1000
+    x = torch.zeros((3, vocab), device="cuda")
+    tokens = torch.arange(10, dtype=torch.int32, device="cuda")
+    off = torch.tensor([-5, 4, 2, 100], dtype=torch.int32, device="cuda")  # before, falling, behind
+    freq = torch.ones(3, device="cuda")
+    out = torch.empty_like(x)
+    tqk.process_logits(tqk.logits_args(x, out=out, tokens=tokens, token_offsets=off, frequency=freq))
+    assert tqk.tqk_device_error_status(tqk.device_status(clear=True)) == tqk.EDEVLEN
+    assert out[0].nonzero()[:, 0].tolist() == [0, 1, 2, 3]
+    assert out[1].nonzero().numel() == 0
+    assert out[2].nonzero()[:, 0].tolist() == list(range(2, 10))
+
+
+def test_captured_with_changing_lists(tqk, cuda):
+    """A captured call replays on whatever the lists and offsets then hold; two graphs side by side."""
+    import torch
+    vocab, rows, cap = 20000, 2, 64
+    rng = np.random.default_rng(2)
+    runs = []
+    for i in range(2):
+        x = torch.from_numpy(rng.standard_normal((rows, vocab), dtype=np.float32)).cuda()
+        out, choice = torch.empty_like(x), torch.empty(rows, dtype=torch.int32, device="cuda")
+        tokens, off = torch.zeros(cap, dtype=torch.int32, device="cuda"), torch.zeros(rows + 1, dtype=torch.int32, device="cuda")
+        rep = torch.full((rows,), 1.5, device="cuda")
+        a = tqk.logits_args(x, out=out, choice=choice, tokens=tokens, token_offsets=off, repetition=rep)
+        tqk.process_logits(a)  # sets the kernel up before the capture
+        s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            tqk.process_logits(a)
+        runs.append((x, out, choice, tokens, off, s, g, rep))
+    for step in range(4):
+        lists = []
+        for x, out, choice, tokens, off, s, g, _ in runs:
+            ids = x.topk(step + 1).indices.to(torch.int32)  # the best tokens are penalised
+            tokens[:rows * (step + 1)] = ids.flatten()
+            off.copy_(torch.arange(rows + 1, dtype=torch.int32) * (step + 1))
+            lists.append(ids.cpu().numpy())
+        torch.cuda.synchronize()
+        for *_, s, g, _ in runs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (x, out, choice, *_), ids in zip(runs, lists):
+            for r in range(rows):
+                ref, best = logits_ref(x[r].cpu().numpy(), tokens=ids[r], repetition=1.5)
+                assert np.array_equal(out[r].cpu().numpy(), ref) and choice[r].item() == best
