@@ -14,13 +14,15 @@
 //      above every weight), into shared memory;
 //   2. the budget-th largest key by radix select, 11 + 11 + 10 bits: a histogram
 //      per CTA in shared memory, summed over the cluster through distributed
-//      shared memory, searched by every CTA alike;
+//      shared memory, searched by every CTA alike.  The third digit only looks at
+//      the keys that share the first two, which the second pass lists;
 //   3. each thread marks the holes (evicted, below `budget`) and movers (kept,
 //      from `budget` on) of its own run of consecutive slots; block and cluster
 //      prefix sums of their counts give every one its rank, and their slots go
 //      into a list that overwrites the keys;
 //   4. the moves are dealt out evenly over the cluster's CTAs, which look up the
-//      j-th hole and the j-th mover in the CTAs' lists and copy the rows.
+//      j-th hole and the j-th mover in the CTAs' lists and copy the rows; every warp
+//      works on moves of its own, 8 of them in flight.
 // Only integer counts are summed, so results do not depend on timing.
 #include "tqk_internal.h"
 
@@ -34,10 +36,15 @@ namespace {
 constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;                   // histogram bins: digits of 11, 11 and 10 bits
-constexpr int EV_BPT = EV_BINS / EV_THREADS;    // bins per thread
 constexpr int EV_RUN_MAX = 63;                  // slots per thread: a bit each of a 64-bit mask, an odd number
-constexpr int EV_CLUSTER_MAX = 16;
-constexpr int EV_BATCH = 128;                   // moves looked up at a time
+constexpr int EV_CLUSTER_MAX = 16;              // non-portable above 8
+constexpr int EV_UNITS = 8;                     // 16-byte units in flight per thread
+constexpr int EV_LOADS = 8;                     // sums and positions in flight per thread
+constexpr int EV_ALONE = 100 << 10;             // dynamic shared memory that leaves no room for a second CTA
+#ifndef EVPER
+#define EVPER 8192
+#endif
+constexpr int EV_STAGE = 8192;                  // slots per CTA whose positions are staged in shared memory
 static_assert(EV_CLUSTER_MAX * EV_THREADS * EV_RUN_MAX == TQK_EVICT_MAX_LEN, "documented limit");
 
 struct EvictParams {
@@ -52,21 +59,21 @@ struct EvictParams {
     const int *position;
     int *position_out;
     long long stat_stride;
-    int run;  // slots per thread at the longest length
+    int run;        // slots per thread at the longest length
+    int staged;     // whether positions are staged: the keys take at most EV_STAGE slots per CTA
+    int *lens_out;  // written here unless it aliases lens, else nullptr
     int *err;
 };
 
 struct EvictShared {
-    unsigned hist[3][EV_BINS];
-    int warp_tot[EV_WARPS];
-    int max_pos;             // this CTA's largest position
-    int counts[2];           // this CTA's holes and movers
-    int ties;                // this CTA's keys equal to the threshold
-    unsigned found_bin;
-    int found_above;
-    int found_count;
+    __align__(16) unsigned hist[3][EV_BINS];
+    int warp_tot[6][EV_WARPS];   // of each block_prefix: a buffer of its own saves a barrier
+    int max_pos;                 // this CTA's largest position
+    int counts[2];               // this CTA's holes and movers
+    int ties;                    // this CTA's keys equal to the threshold
+    int n_close;                 // keys that share the first two digits
+    int found[3][3];             // per digit: the bin of the budget-th key, how many keys lie above it, its own
     int pre_h[EV_CLUSTER_MAX + 1], pre_m[EV_CLUSTER_MAX + 1];
-    int src[EV_BATCH], dst[EV_BATCH];
 };
 
 // A float's bits reordered so that unsigned comparison orders them: negative numbers below positive ones,
@@ -78,7 +85,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 constexpr uint32_t KEY_PROTECTED = 0xFFFFFFFFu;  // above +inf's 0xFF800000
 
-// Exclusive prefix sum of v over the CTA's threads; *total receives the sum.  Ends with a barrier.
+// Exclusive prefix sum of v over the CTA's threads; *total receives the sum.  warp_tot: a buffer that no other call uses.
 __device__ __forceinline__ int block_prefix(int v, int *warp_tot, int *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int incl = v;
@@ -89,68 +96,81 @@ __device__ __forceinline__ int block_prefix(int v, int *warp_tot, int *total) {
     }
     if (lane == 31) warp_tot[warp] = incl;
     __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < EV_WARPS; w++) {
-        const int x = warp_tot[w];
-        if (w < warp) before += x;
-        all += x;
-    }
-    __syncthreads();
-    *total = all;
+    // the warps' totals, one per lane
+    int before = lane < EV_WARPS ? warp_tot[lane] : 0, all = before;
+    if (lane >= warp) before = 0;
+    before = __reduce_add_sync(0xffffffffu, before);
+    *total = __reduce_add_sync(0xffffffffu, all);
     return before + incl - v;
 }
 
-// Copies moves [0, n) of sh.src / sh.dst: whole rows of both planes.
+// One warp moves rows of both planes from slots src to slots dst, lane l's move in its src and dst, the first n lanes'.
+// A row is 9 16-byte units (9 words for head_dim 32), or twice as many; K's and V's units lie next to each other in the
+// lanes where both fit, so a lane's place in the row never changes and a move costs one load and one store.  Denser
+// layouts (every lane at work, twice the bytes in flight) were slower: 128 us against 119 us for a ragged batch.
 template <int NB>
-__device__ __forceinline__ void copy_rows(uint8_t *kh, uint8_t *vh, const EvictShared &sh, int n) {
+__device__ __forceinline__ void move_rows(uint8_t *kh, uint8_t *vh, int src, int dst, int n) {
     constexpr int ROW = NB * BLOCK_BYTES;
     using Unit = typename std::conditional<NB % 4 == 0, uint4, uint32_t>::type;  // rows of 4 blocks are 16-byte aligned
-    constexpr int UNITS = ROW / (int)sizeof(Unit);
-    constexpr int IN_FLIGHT = 4;
-    const int total = n * 2 * UNITS;
-    for (int i0 = threadIdx.x; i0 < total; i0 += IN_FLIGHT * EV_THREADS) {
-        Unit x[IN_FLIGHT];
-        Unit *to[IN_FLIGHT];
+    constexpr int UNITS = ROW / (int)sizeof(Unit);   // 9 or 18
+    constexpr int LOADS = UNITS == 9 ? 1 : 2;        // per move
+    constexpr int MOVES = EV_UNITS / LOADS;          // in flight
+    const int lane = threadIdx.x & 31;
+    const bool active = lane < 18;
+    uint8_t *base[LOADS];
 #pragma unroll
-        for (int q = 0; q < IN_FLIGHT; q++) {
-            const int i = i0 + q * EV_THREADS;
-            if (i >= total) break;
-            const int row = i / UNITS, u = i - row * UNITS, m = row >> 1;
-            uint8_t *plane = row & 1 ? vh : kh;
-            x[q] = reinterpret_cast<const Unit *>(plane + (long long)sh.src[m] * ROW)[u];
-            to[q] = reinterpret_cast<Unit *>(plane + (long long)sh.dst[m] * ROW) + u;
+    for (int l = 0; l < LOADS; l++)
+        base[l] = LOADS == 2 ? (l ? vh : kh) + lane * sizeof(Unit)
+                             : lane < 9 ? kh + lane * sizeof(Unit) : vh + (lane - 9) * sizeof(Unit);
+    for (int m0 = 0; m0 < n; m0 += MOVES) {
+        Unit x[MOVES][LOADS];
+#pragma unroll
+        for (int q = 0; q < MOVES; q++) {
+            const long long from = (long long)__shfl_sync(0xffffffffu, src, m0 + q) * ROW;
+#pragma unroll
+            for (int l = 0; l < LOADS; l++)
+                if (active && m0 + q < n) x[q][l] = *reinterpret_cast<const Unit *>(base[l] + from);
         }
 #pragma unroll
-        for (int q = 0; q < IN_FLIGHT; q++)
-            if (i0 + q * EV_THREADS < total) *to[q] = x[q];
+        for (int q = 0; q < MOVES; q++) {
+            const long long to = (long long)__shfl_sync(0xffffffffu, dst, m0 + q) * ROW;
+#pragma unroll
+            for (int l = 0; l < LOADS; l++)
+                if (active && m0 + q < n) *reinterpret_cast<Unit *>(base[l] + to) = x[q][l];
+        }
     }
 }
 
 template <int NB>
-__global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t keys[];  // [EV_THREADS * run], then the slots of holes and movers
     __shared__ EvictShared sh;
+    const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x;
+    for (int i = tid; i < 3 * EV_BINS / 4; i += EV_THREADS) reinterpret_cast<uint4 *>(sh.hist)[i] = uint4{0, 0, 0, 0};
+    if (tid == 0) {
+        sh.max_pos = INT_MIN;
+        sh.n_close = 0;
+    }
+    __syncthreads();
     grid_dependency_wait();
     grid_dependents_launch();
-    const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x;
     const int kvh = blockIdx.y, item = blockIdx.z;
     int len = p.lens ? p.lens[item] : p.len0 + item * p.len_step;
     if (len < 0 || len > p.len_cap) {
         if (tid == 0) record_error(p.err, DEVERR_BADLEN);
         len = len < 0 ? 0 : p.len_cap;
     }
+    const int budget = p.budget;
+    if (p.lens_out && rank == 0 && kvh == 0 && tid == 0) p.lens_out[item] = min(len, budget);
     const long long at = (long long)item * p.stat_stride + (long long)kvh * p.max_tokens;
     const float *w_in = p.weight + at;
     float *w_out = p.weight_out + at;
     const int *pos_in = p.position ? p.position + at : nullptr;
     int *pos_out = p.position ? p.position_out + at : nullptr;
     const bool copy_w = w_out != w_in, copy_pos = pos_out != pos_in;
-    const int budget = p.budget;
     // this CTA's slots [s0, s1), `run` consecutive ones per thread; an odd run keeps the threads' shared-memory
     // words in different banks
-    const int per = (len + C * EV_THREADS - 1) / (C * EV_THREADS);
-    const int run = per | 1;
+    const int run = ((len + C * EV_THREADS - 1) / (C * EV_THREADS)) | 1;
     const int s0 = min(len, rank * run * EV_THREADS), s1 = min(len, s0 + run * EV_THREADS), n_own = s1 - s0;
     auto cluster_barrier = [&]() {
         if (C > 1) cluster_sync_all();
@@ -165,83 +185,120 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictParams p) 
         return;
     }
 
-    // ---- 1. keys
-    for (int i = tid; i < 3 * EV_BINS; i += EV_THREADS) (&sh.hist[0][0])[i] = 0;
-    int newest = 0;
-    if (p.n_recent > 0) {
-        int m = INT_MIN;
-        for (int i = s0 + tid; i < s1; i += EV_THREADS) m = max(m, pos_in[i]);
-        m = __reduce_max_sync(0xffffffffu, m);
-        if ((tid & 31) == 0) sh.warp_tot[tid >> 5] = m;
-        __syncthreads();
-        if (tid < 32) {
-            m = __reduce_max_sync(0xffffffffu, tid < EV_WARPS ? sh.warp_tot[tid] : INT_MIN);
-            if (tid == 0) sh.max_pos = m;
+    // ---- 1. keys.  Protection needs the newest position first: the positions wait in shared memory behind the keys,
+    //         or, from EV_STAGE slots per CTA on, are read again
+    const bool recent = p.n_recent > 0, staged = p.staged;
+    int *pos_s = reinterpret_cast<int *>(keys) + EV_THREADS * p.run;
+    int newest = INT_MIN;
+    for (int i0 = tid; i0 < n_own; i0 += EV_LOADS * EV_THREADS) {
+        float w[EV_LOADS];
+        int pos[EV_LOADS];
+#pragma unroll
+        for (int q = 0; q < EV_LOADS; q++) {
+            const int s = s0 + i0 + q * EV_THREADS;
+            w[q] = s < s1 ? w_in[s] : 0.0f;
+            pos[q] = pos_in && s < s1 ? pos_in[s] : INT_MIN;
         }
+#pragma unroll
+        for (int q = 0; q < EV_LOADS; q++) {
+            const int i = i0 + q * EV_THREADS, s = s0 + i;
+            if (i >= n_own) break;
+            newest = max(newest, pos[q]);
+            keys[i] = pos_in && pos[q] < p.n_first ? KEY_PROTECTED : weight_key(w[q]);
+            if (recent && staged) pos_s[i] = pos[q];
+            if (s < budget) {
+                if (copy_w) w_out[s] = w[q];
+                if (copy_pos) pos_out[s] = pos[q];
+            }
+        }
+    }
+    if (recent) {
+        newest = __reduce_max_sync(0xffffffffu, newest);
+        if ((tid & 31) == 0) atomicMax(&sh.max_pos, newest);
         cluster_barrier();
-        newest = INT_MIN;
-        for (int r = 0; r < C; r++)
-            newest = max(newest, C > 1 ? (int)ld_cluster_u32(cluster_map(&sh.max_pos, r)) : sh.max_pos);
+        newest = (int)ld_cluster_u32(cluster_map(&sh.max_pos, (uint32_t)min(tid & 31, C - 1)));
+        newest = __reduce_max_sync(0xffffffffu, newest);
     }
+    // the first digit's histogram, from the final keys (each thread its own slots')
     const long long recent_from = (long long)newest - p.n_recent;  // positions above are protected
-    for (int i = tid; i < n_own; i += EV_THREADS) {
-        const int s = s0 + i;
-        const float w = w_in[s];
-        uint32_t key = weight_key(w);
-        if (pos_in) {
-            const int pos = pos_in[s];
-            if (pos < p.n_first || (p.n_recent > 0 && pos > recent_from)) key = KEY_PROTECTED;
-            if (copy_pos && s < budget) pos_out[s] = pos;
+    for (int i0 = tid; i0 < n_own; i0 += EV_LOADS * EV_THREADS) {
+        int pos[EV_LOADS];
+        if (recent) {
+#pragma unroll
+            for (int q = 0; q < EV_LOADS; q++) {
+                const int i = i0 + q * EV_THREADS;
+                pos[q] = i >= n_own ? INT_MIN : staged ? pos_s[i] : pos_in[s0 + i];
+            }
         }
-        if (copy_w && s < budget) w_out[s] = w;
-        keys[i] = key;
+#pragma unroll
+        for (int q = 0; q < EV_LOADS; q++) {
+            const int i = i0 + q * EV_THREADS;
+            if (i >= n_own) break;
+            uint32_t key = keys[i];
+            if (recent && pos[q] > recent_from) keys[i] = key = KEY_PROTECTED;
+            atomicAdd(&sh.hist[0][key >> 21], 1u);
+        }
     }
-    __syncthreads();
 
     // ---- 2. the budget-th largest key: `prefix` holds its digits found so far, `need` of the keys that share
     //         them are kept
     uint32_t prefix = 0;
     int need = budget, equal = 0;
+    uint32_t *close = reinterpret_cast<uint32_t *>(pos_s);  // the keys that share two digits, as far as they fit
+    const int close_cap = staged ? EV_THREADS * p.run : 0;
 #pragma unroll
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        const int bins = 1 << bits;
-        unsigned *hist = sh.hist[pass];
-        for (int i = tid; i < n_own; i += EV_THREADS) {
-            const uint32_t key = keys[i];
-            if (pass == 0 || (key >> (shift + bits)) == (prefix >> (shift + bits)))
-                atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
+    for (int digit = 0; digit < 3; digit++) {
+        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bins = digit == 2 ? 1024 : 2048;
+        unsigned *hist = sh.hist[digit];
+        if (digit == 1) {
+            for (int i = tid; i < n_own; i += EV_THREADS) {
+                const uint32_t key = keys[i];
+                if (key >> 21 != prefix >> 21) continue;
+                atomicAdd(&hist[(key >> 10) & 2047], 1u);
+                const int at_close = atomicAdd(&sh.n_close, 1);
+                if (at_close < close_cap) close[at_close] = key;
+            }
+        } else if (digit == 2) {
+            const bool listed = sh.n_close <= close_cap;
+            const uint32_t *from = listed ? close : keys;
+            const int n = listed ? sh.n_close : n_own;
+            for (int i = tid; i < n; i += EV_THREADS)
+                if (from[i] >> 10 == prefix >> 10) atomicAdd(&hist[from[i] & 1023], 1u);
         }
         cluster_barrier();
-        // thread `tid` counts the bins from the top: descending order, EV_BPT (half as many in the last pass) each
-        const int bpt = bins / EV_THREADS;
-        int cnt[EV_BPT], sum = 0;
-#pragma unroll
-        for (int q = 0; q < EV_BPT; q++) {
-            cnt[q] = 0;
-            if (q < bpt) {
-                const int bin = bins - 1 - (tid * bpt + q);
-                if (C == 1) cnt[q] = (int)hist[bin];
-                else
-                    for (int r = 0; r < C; r++) cnt[q] += (int)ld_cluster_u32(cluster_map(&hist[bin], r));
+        // over the cluster: each CTA adds the others' counts of its share of the bins to its own, four bins of one
+        // CTA per thread, and then everyone reads every share
+        const int share = bins / C;  // C is a power of two
+        if (C > 1) {
+            const int r = tid / (share / 4), bin = rank * share + 4 * (tid % (share / 4));
+            if (r < C && r != rank) {
+                const uint4 x = ld_cluster_u32x4(cluster_map(hist + bin, (uint32_t)r));
+                if (x.x) atomicAdd(&hist[bin], x.x);
+                if (x.y) atomicAdd(&hist[bin + 1], x.y);
+                if (x.z) atomicAdd(&hist[bin + 2], x.z);
+                if (x.w) atomicAdd(&hist[bin + 3], x.w);
             }
-            sum += cnt[q];
+            cluster_sync_all();
         }
-        int all, above = block_prefix(sum, sh.warp_tot, &all);
+        // thread t takes the t-th four bins from the top
+        uint4 cnt{0, 0, 0, 0};
+        const int bin0 = bins - 4 - 4 * tid;
+        if (bin0 >= 0) cnt = ld_cluster_u32x4(cluster_map(hist + bin0, (uint32_t)(bin0 / share)));
+        int all, above = block_prefix((int)(cnt.x + cnt.y + cnt.z + cnt.w), sh.warp_tot[digit], &all);
+        const int c4[4] = {(int)cnt.w, (int)cnt.z, (int)cnt.y, (int)cnt.x};
 #pragma unroll
-        for (int q = 0; q < EV_BPT; q++) {
-            if (q < bpt && above < need && need <= above + cnt[q]) {
-                sh.found_bin = (unsigned)(bins - 1 - (tid * bpt + q));
-                sh.found_above = above;
-                sh.found_count = cnt[q];
+        for (int q = 0; q < 4; q++) {
+            if (above < need && need <= above + c4[q]) {
+                sh.found[digit][0] = bin0 + 3 - q;
+                sh.found[digit][1] = above;
+                sh.found[digit][2] = c4[q];
             }
-            above += cnt[q];
+            above += c4[q];
         }
         __syncthreads();
-        prefix |= sh.found_bin << shift;
-        need -= sh.found_above;
-        equal = sh.found_count;
-        __syncthreads();
+        prefix |= (uint32_t)sh.found[digit][0] << shift;
+        need -= sh.found[digit][1];
+        equal = sh.found[digit][2];
     }
 
     // ---- 3. holes and movers of this thread's run
@@ -250,10 +307,14 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictParams p) 
     if (equal > need) {
         int ties = 0, all;
         for (int i = r0; i < r1; i++) ties += keys[i] == prefix;
-        tie_rank = block_prefix(ties, sh.warp_tot, &all);
-        if (tid == 0) sh.ties = all;
-        cluster_barrier();
-        for (int r = 0; r < rank; r++) tie_rank += (int)ld_cluster_u32(cluster_map(&sh.ties, r));
+        tie_rank = block_prefix(ties, sh.warp_tot[3], &all);
+        if (C > 1) {
+            if (tid == 0) sh.ties = all;
+            cluster_sync_all();
+            const int r = tid & 31;
+            const int x = r < rank ? (int)ld_cluster_u32(cluster_map(&sh.ties, (uint32_t)r)) : 0;
+            tie_rank += __reduce_add_sync(0xffffffffu, x);
+        }
     }
     unsigned long long holes = 0, movers = 0;
     for (int i = r0; i < r1; i++) {
@@ -264,28 +325,38 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictParams p) 
         if (s0 + i < budget) holes |= keep ? 0ull : bit;
         else movers |= keep ? bit : 0ull;
     }
-    // at most 16 * 63 slots per warp and 32256 per CTA: both counts fit in half a word
-    int all;
-    const int at2 = block_prefix((__popcll(holes) << 16) | __popcll(movers), sh.warp_tot, &all);
+    // at most 32256 slots per CTA: both counts fit in half a word
+    int both;
+    const int ranks = block_prefix((__popcll(holes) << 16) | __popcll(movers), sh.warp_tot[4], &both);
     int *list = reinterpret_cast<int *>(keys);  // every key is read: holes from the front, movers from the back
     const int last = EV_THREADS * run - 1;
-    for (int j = at2 >> 16; holes; holes &= holes - 1) list[j++] = s0 + r0 + __ffsll(holes) - 1;
-    for (int j = at2 & 0xFFFF; movers; movers &= movers - 1) list[last - j++] = s0 + r0 + __ffsll(movers) - 1;
+    for (int j = ranks >> 16; holes; holes &= holes - 1) list[j++] = s0 + r0 + __ffsll(holes) - 1;
+    for (int j = ranks & 0xFFFF; movers; movers &= movers - 1) list[last - j++] = s0 + r0 + __ffsll(movers) - 1;
     if (tid == 0) {
-        sh.counts[0] = all >> 16;
-        sh.counts[1] = all & 0xFFFF;
+        sh.counts[0] = both >> 16;
+        sh.counts[1] = both & 0xFFFF;
     }
     cluster_barrier();
-    if (tid == 0) {
+    if (tid < 32) {  // exclusive prefixes over the cluster, lane r for CTA r
         int h = 0, m = 0;
-        for (int r = 0; r < C; r++) {
-            sh.pre_h[r] = h;
-            sh.pre_m[r] = m;
-            h += C > 1 ? (int)ld_cluster_u32(cluster_map(&sh.counts[0], r)) : sh.counts[0];
-            m += C > 1 ? (int)ld_cluster_u32(cluster_map(&sh.counts[1], r)) : sh.counts[1];
+        if (tid < C) {
+            h = (int)ld_cluster_u32(cluster_map(&sh.counts[0], (uint32_t)tid));
+            m = (int)ld_cluster_u32(cluster_map(&sh.counts[1], (uint32_t)tid));
         }
-        sh.pre_h[C] = h;
-        sh.pre_m[C] = m;
+        int hi = h, mi = m;
+#pragma unroll
+        for (int o = 1; o < EV_CLUSTER_MAX; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, hi, o), y = __shfl_up_sync(0xffffffffu, mi, o);
+            if (tid >= o) {
+                hi += x;
+                mi += y;
+            }
+        }
+        if (tid < C) {
+            sh.pre_h[tid + 1] = hi;
+            sh.pre_m[tid + 1] = mi;
+        }
+        if (tid == 0) sh.pre_h[0] = sh.pre_m[0] = 0;
     }
     __syncthreads();
 
@@ -293,31 +364,29 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictParams p) 
     const long long n_moves = sh.pre_m[C];
     const int m0 = (int)(n_moves * rank / C), m1 = (int)(n_moves * (rank + 1) / C);
     const long long head_off = (long long)item * p.item_stride + (long long)kvh * p.max_tokens * (NB * BLOCK_BYTES);
-    for (int b = m0; b < m1; b += EV_BATCH) {
-        const int n = min(EV_BATCH, m1 - b);
-        if (tid < 2 * n) {
-            // the first n threads look up the holes, the next n the movers
-            const bool mover = tid >= n;
-            const int j = b + (mover ? tid - n : tid);
-            const int *pre = mover ? sh.pre_m : sh.pre_h;
-            int r = 0;
-            while (r + 1 < C && pre[r + 1] <= j) r++;
-            const int *slot = mover ? &list[last - (j - pre[r])] : &list[j - pre[r]];
-            const int v = C > 1 ? (int)ld_cluster_u32(cluster_map(slot, r)) : *slot;
-            (mover ? sh.src : sh.dst)[j - b] = v;
+    // up to 32 moves at a time per warp, a lane looking each of them up
+    auto slot_of = [&](const int *pre, int j, bool mover) {
+        int r = 0;
+        while (r + 1 < C && pre[r + 1] <= j) r++;
+        return (int)ld_cluster_u32(cluster_map(mover ? &list[last - (j - pre[r])] : &list[j - pre[r]], (uint32_t)r));
+    };
+    // few moves are spread over the warps
+    const int lane = tid & 31, step = max(1, min(32, (m1 - m0 + EV_WARPS - 1) / EV_WARPS));
+    for (int b = m0 + (tid >> 5) * step; b < m1; b += EV_WARPS * step) {
+        const int n = min(step, m1 - b);
+        int src = 0, dst = 0;
+        if (lane < n) {
+            src = slot_of(sh.pre_m, b + lane, true);
+            dst = slot_of(sh.pre_h, b + lane, false);
+            w_out[dst] = w_in[src];
+            if (pos_in) pos_out[dst] = pos_in[src];
         }
-        __syncthreads();
-        if (tid < n) {
-            w_out[sh.dst[tid]] = w_in[sh.src[tid]];
-            if (pos_in) pos_out[sh.dst[tid]] = pos_in[sh.src[tid]];
-        }
-        copy_rows<NB>(p.k + head_off, p.v + head_off, sh, n);
-        __syncthreads();
+        move_rows<NB>(p.k + head_off, p.v + head_off, src, dst, n);
     }
     if (C > 1) cluster_sync_all();  // no CTA leaves while another reads its list
 }
 
-// lens_out[i] = min(len_i, budget), after the eviction has read every length.
+// lens_out[i] = min(len_i, budget) in place: after the eviction has read every length.
 __global__ void evict_lens_kernel(const int *lens, int len0, int len_step, int len_cap, int budget, int n, int *out) {
     grid_dependency_wait();
     grid_dependents_launch();
@@ -327,7 +396,9 @@ __global__ void evict_lens_kernel(const int *lens, int len0, int len_step, int l
 
 template <int NB>
 int launch_evict(const EvictParams &p, int cluster, dim3 grid, cudaStream_t stream) {
-    const size_t smem = (size_t)EV_THREADS * p.run * sizeof(uint32_t);
+    size_t smem = (size_t)EV_THREADS * p.run * (p.staged ? 2 : 1) * sizeof(uint32_t);
+    // few CTAs: one per SM (two would share an SM while others idle); the largest clusters do not fit a GPC that way
+    if (cluster <= 8 && (long long)grid.x * grid.y * grid.z <= device_info()->sm_count && smem < EV_ALONE) smem = EV_ALONE;
     // the shared-memory and cluster-size opt-ins are per-device function attributes
     static std::mutex mu;
     static bool ready[64];
@@ -416,11 +487,13 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
         p.position_out = a->position_out;
         p.stat_stride = a->stat_item_stride;
         p.err = device_info()->err_word;
-        // CTAs per (item, head): a portable cluster of 8 for lengths that need more than one CTA's 8192 slots,
-        // 16 where 8 do not hold the keys
-        int cluster = (max_len + 8191) / 8192;
-        if (cluster > 8) cluster = max_len > 8 * EV_THREADS * EV_RUN_MAX ? EV_CLUSTER_MAX : 8;
+        // CTAs per (item, head): one up to 8192 slots (clusters cost more than they bring there), then as many as hold
+        // 8192 each, as far as a cluster goes
+        int cluster = 1;
+        while (cluster < EV_CLUSTER_MAX && cluster * EVPER < max_len) cluster *= 2;
         p.run = ((max_len + cluster * EV_THREADS - 1) / (cluster * EV_THREADS)) | 1;
+        p.staged = max_len <= cluster * EV_STAGE;
+        p.lens_out = a->lens_out != a->lens ? a->lens_out : nullptr;
         const dim3 grid((unsigned)cluster, (unsigned)a->n_kv_heads, (unsigned)a->n_items);
         switch (nb) {
             case 1: rc = launch_evict<1>(p, cluster, grid, st); break;
@@ -430,7 +503,7 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
         }
         if (rc) return rc;
     }
-    if (!a->lens_out) return TQK_OK;
+    if (!a->lens_out || (max_len > 0 && a->lens_out != a->lens)) return TQK_OK;
     return launch_pdl(evict_lens_kernel, dim3((unsigned)((a->n_items + 255) / 256)), dim3(256), 0, st, a->lens, a->len0,
                       a->len_step, max_len, a->budget, a->n_items, a->lens_out);
 }

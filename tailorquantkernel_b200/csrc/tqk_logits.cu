@@ -2,28 +2,55 @@
 // repetition, frequency and presence penalties over each row's history, token
 // biases, a grammar's bit mask, and the greedy choice among what is left.
 //
-// One thread-block cluster per row, a contiguous part of the vocabulary per CTA,
-// worked through in pieces of LG_PIECE tokens: the piece's logits are loaded into
-// registers first (8 16-byte loads in flight per thread); while they are on
-// their way, the row's history is scanned and the piece's tokens are counted in
-// shared memory (a word per token: bit 31 seen, bit 30 in the bias list, the rest
-// the count after the prompt; integer atomics, so the order does not show); then
-// penalties, biases and mask are applied in registers and the piece is stored
-// once.  Every logit is read and written once: 8 bytes of DRAM traffic per token
-// bound the kernel, and the history costs 4 bytes per entry and CTA, from L2.
-// The CTAs' largest values meet through distributed shared memory.
+// One thread-block cluster per row; blocks of 128 tokens are dealt out to its
+// CTAs in turn.  The bulk of a row -- tokens in neither its history nor its bias
+// list -- only meets the mask and is streamed through registers: 8 16-byte loads
+// in flight per thread, each logit read and written once, which is the kernel's
+// floor (8 bytes of DRAM traffic per token).  Around the stream:
+//   * while the first logits are on their way, every CTA scans the history and
+//     counts its own tokens in shared memory (a counter per token: seen, in the
+//     bias list, and the count after the prompt; integer atomics, so their order
+//     does not show).  Frequent tokens have neighbouring ids in many vocabularies;
+//     dealing out small blocks spreads them over the CTAs;
+//   * the stream leaves counted tokens alone and puts them on a list; the list is
+//     worked off with full warps, so the division and the branches of the
+//     penalties cost by the distinct tokens of the history, not by the vocabulary;
+//     the next logits are loaded meanwhile;
+//   * each CTA pushes its candidate for the greedy choice to the first CTA's
+//     shared memory and leaves.
 #include "tqk_internal.h"
 
+#include <climits>
 #include <mutex>
 
 namespace tqk {
 namespace {
 
-constexpr int LG_THREADS = 512;
-constexpr int LG_PER_THREAD = 32;                        // logits per thread and piece, in registers
-constexpr int LG_PIECE = LG_THREADS * LG_PER_THREAD;     // 16384 tokens
-constexpr int LG_CLUSTER = 8;                            // most CTAs per row (portable cluster size)
-constexpr uint32_t LG_SEEN = 0x80000000u, LG_BIASED = 0x40000000u, LG_COUNT = 0x3FFFFFFFu;
+constexpr int LG_THREADS = 256;
+constexpr int LG_WARPS = LG_THREADS / 32;
+constexpr int LG_BLOCK = 128;                            // tokens per block: a warp's 16-byte loads
+constexpr int LG_LOADS = 8;                              // blocks per warp and chunk, in registers
+constexpr int LG_CHUNK = LG_WARPS * LG_LOADS * LG_BLOCK; // 8192 tokens
+constexpr int LG_CLUSTER = 16;                           // most CTAs per row (non-portable above 8), a power of two
+constexpr int LG_COUNT_BYTES_MAX = 64 << 10;             // counters per CTA
+constexpr int LG_SCAN = 8;                               // history entries in flight per thread
+
+// Counters: 16 bits per token (two to a word) for histories of up to LG_SHORT entries, else 32 bits.  From the top:
+// seen, in the bias list, more than once in the bias list, and the count after the prompt.
+constexpr int LG_SHORT = (1 << 13) - 1;
+template <bool SHORT>
+struct Counter {
+    static constexpr int BITS = SHORT ? 16 : 32;
+    static constexpr uint32_t SEEN = 1u << (BITS - 1), BIASED = 1u << (BITS - 2), AGAIN = 1u << (BITS - 3);
+    static constexpr uint32_t COUNT = AGAIN - 1;
+    // the word of token t, and the place of its counter in it
+    static __device__ __forceinline__ int word(int t) { return SHORT ? t >> 1 : t; }
+    static __device__ __forceinline__ int shift(int t) { return SHORT ? (t & 1) * 16 : 0; }
+    static __device__ __forceinline__ uint32_t get(const uint32_t *c, int t) {
+        return SHORT ? (c[t >> 1] >> shift(t)) & 0xFFFFu : c[t];
+    }
+};
+constexpr int LG_COUNT_MAX = Counter<false>::COUNT;
 
 struct LogitsParams {
     const float *logits;
@@ -44,7 +71,9 @@ struct LogitsParams {
     long long mask_stride;
     const int *mask_rows;
     int n_mask_rows;
-    int per_cta;  // tokens per CTA, a multiple of 128
+    int log_c;        // log2 of the CTAs per row
+    int own_blocks;   // blocks per CTA
+    int count_bytes;  // counters' shared memory, whole chunks
     int *err;
 };
 
@@ -66,166 +95,305 @@ __device__ __forceinline__ Best better(Best a, Best b) {
     return take ? b : a;
 }
 
+// What all threads of a CTA know of their row.
+struct Row {
+    const float *src;
+    float *dst;
+    const uint32_t *mask;  // or nullptr
+    bool barred;           // a bad mask row index: nothing is allowed
+    int h0, h1, prompt_end, b0, b1;
+};
+
+// Bit t of the row's mask.
+__device__ __forceinline__ bool allowed_token(const Row &r, int t) {
+    return !r.barred && (!r.mask || (r.mask[t >> 5] >> (t & 31)) & 1u);
+}
+
+// A listed token's final value: penalties by its counter c, then its biases' sum s.
+template <bool SHORT>
+__device__ __forceinline__ float constrained(const LogitsParams &p, const Row &r, int row, int t, uint32_t c, float s) {
+    using K = Counter<SHORT>;
+    float v = r.src[t];  // in place: still the logit
+    if (p.repetition && (c & (K::SEEN | K::COUNT))) {
+        const float rep = p.repetition[row];
+        v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+    }
+    if (c & K::COUNT) {
+        const float freq = p.frequency ? p.frequency[row] : 0.0f, pres = p.presence ? p.presence[row] : 0.0f;
+        v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, __uint2float_rn(c & K::COUNT))), pres);
+    }
+    if (c & K::BIASED) v = __fadd_rn(v, s);
+    return allowed_token(r, t) ? v : -INFINITY;
+}
+
+// The CTA's tokens: block b of the row is block b >> log_c of CTA b mod C.  The row's token at place i of them:
+__device__ __forceinline__ int token_at(const LogitsParams &p, int i) {
+    return (((i / LG_BLOCK) << p.log_c) + (int)blockIdx.x) * LG_BLOCK + i % LG_BLOCK;
+}
+// ... and the place of token `tok`, or -1 when it is another CTA's or outside the vocabulary.
+__device__ __forceinline__ int place_of(const LogitsParams &p, int tok) {
+    const int blk = tok / LG_BLOCK;
+    if ((unsigned)tok >= (unsigned)p.vocab || (blk & ((1 << p.log_c) - 1)) != (int)blockIdx.x) return -1;
+    return (blk >> p.log_c) * LG_BLOCK + tok % LG_BLOCK;
+}
+
+// The logits of the chunk at place t0, 8 blocks per warp.  VEC: tokens 4 lane .. 4 lane + 3 of each block; else tokens
+// lane, 32 + lane, 64 + lane, 96 + lane.
+template <bool VEC>
+__device__ __forceinline__ void load_chunk(const LogitsParams &p, const float *src, int t0, float (&x)[LG_LOADS][4]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int k = 0; k < LG_LOADS; k++) {
+        const int first = token_at(p, t0 + (warp + k * LG_WARPS) * LG_BLOCK);
+        if constexpr (VEC) {
+            const int t = first + 4 * lane;
+            if (t + 4 <= p.vocab) {
+                const float4 f = *reinterpret_cast<const float4 *>(src + t);
+                x[k][0] = f.x; x[k][1] = f.y; x[k][2] = f.z; x[k][3] = f.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[k][j] = t + j < p.vocab ? src[t + j] : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[k][j] = first + 32 * j + lane < p.vocab ? src[first + 32 * j + lane] : 0.0f;
+        }
+    }
+}
+// The warp's 32 mask words of the chunk, lane l holding word l % 4 of block l / 4.
+__device__ __forceinline__ uint32_t load_words(const LogitsParams &p, const Row &r, int t0) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t words = r.barred ? 0u : 0xFFFFFFFFu;
+    if (r.mask) {
+        const int t = token_at(p, t0 + (warp + (lane >> 2) * LG_WARPS) * LG_BLOCK) + 32 * (lane & 3);
+        if (t < p.vocab) words = r.mask[t >> 5];
+    }
+    return words;
+}
+
+// This CTA's share of a row.  On entry x holds the first chunk, and the counters, which cover `span` tokens (whole
+// chunks) at a time, and both list lengths are zero.
+template <bool VEC, bool COUNT, bool SHORT>
+__device__ __forceinline__ Best work_row(const LogitsParams &p, const Row &r, int row, int span, uint32_t *counts,
+                                         uint16_t *list, int *n_listed, float (&x)[LG_LOADS][4]) {
+    using K = Counter<SHORT>;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int own = p.own_blocks * LG_BLOCK;
+    Best best{-INFINITY, -1};
+    uint32_t words = load_words(p, r, 0);
+    for (int t0 = 0, c0 = 0, chunk = 0; t0 < own; t0 += LG_CHUNK, chunk++) {
+        if constexpr (COUNT) {
+            if (t0 == 0 || t0 == c0 + span) {
+                // ---- the counters of the tokens from t0 on
+                if (t0 > 0) {  // the last span's are done with (the barrier after its last list)
+                    for (int i = tid; i < p.count_bytes / 16; i += LG_THREADS)
+                        reinterpret_cast<uint4 *>(counts)[i] = uint4{0, 0, 0, 0};
+                }
+                c0 = t0;
+                __syncthreads();
+                for (int i0 = r.h0 + tid; i0 < r.h1; i0 += LG_SCAN * LG_THREADS) {
+                    int tok[LG_SCAN];
+#pragma unroll
+                    for (int q = 0; q < LG_SCAN; q++) {
+                        const int i = i0 + q * LG_THREADS;
+                        tok[q] = i < r.h1 ? p.tokens[i] : -1;
+                    }
+#pragma unroll
+                    for (int q = 0; q < LG_SCAN; q++) {
+                        const int t = place_of(p, tok[q]) - c0;
+                        if ((unsigned)t >= (unsigned)span) continue;
+                        if (i0 + q * LG_THREADS < r.prompt_end) atomicOr(&counts[K::word(t)], K::SEEN << K::shift(t));
+                        else atomicAdd(&counts[K::word(t)], 1u << K::shift(t));
+                    }
+                }
+                for (int i = r.b0 + tid; i < r.b1; i += LG_THREADS) {
+                    const int t = place_of(p, p.bias_tokens[i]) - c0;
+                    if ((unsigned)t >= (unsigned)span) continue;
+                    const uint32_t flag = K::BIASED << K::shift(t);
+                    if (atomicOr(&counts[K::word(t)], flag) & flag) atomicOr(&counts[K::word(t)], K::AGAIN << K::shift(t));
+                }
+                __syncthreads();
+            }
+        }
+        // ---- the stream: counted tokens keep their logit for now
+#pragma unroll
+        for (int k = 0; k < LG_LOADS; k++) {
+            const int i = (warp + k * LG_WARPS) * LG_BLOCK;  // the block's place in the chunk
+            const int first = token_at(p, t0 + i);
+            uint32_t bits = 0;
+            if constexpr (VEC) bits = __shfl_sync(0xffffffffu, words, k * 4 + (lane >> 3)) >> (4 * (lane & 7));
+            uint32_t c[4] = {};
+            if constexpr (COUNT) {
+                const int at = t0 - c0 + i;
+                if constexpr (!VEC) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) c[j] = K::get(counts, at + 32 * j + lane);
+                } else if constexpr (SHORT) {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(counts + (at + 4 * lane) / 2);
+                    c[0] = u.x & 0xFFFFu; c[1] = u.x >> 16; c[2] = u.y & 0xFFFFu; c[3] = u.y >> 16;
+                } else {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(counts + at + 4 * lane);
+                    c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int in = VEC ? 4 * lane + j : 32 * j + lane;
+                bool allowed;
+                if constexpr (VEC) allowed = (bits >> j) & 1u;
+                else allowed = (__shfl_sync(0xffffffffu, words, k * 4 + j) >> lane) & 1u;
+                if (COUNT && c[j]) {
+                    list[atomicAdd(&n_listed[chunk & 1], 1)] = (uint16_t)(i + in);
+                } else {
+                    if (!allowed) x[k][j] = -INFINITY;
+                    if (x[k][j] > best.v && first + in < p.vocab) best = Best{x[k][j], first + in};
+                }
+            }
+            if (!r.dst) continue;
+            if constexpr (VEC) {
+                const int t = first + 4 * lane;
+                if (t + 4 <= p.vocab) {
+                    *reinterpret_cast<float4 *>(r.dst + t) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (t + j < p.vocab) r.dst[t + j] = x[k][j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (first + 32 * j + lane < p.vocab) r.dst[first + 32 * j + lane] = x[k][j];
+            }
+        }
+        const bool more = t0 + LG_CHUNK < own;
+        if (more) {
+            load_chunk<VEC>(p, r.src, t0 + LG_CHUNK, x);
+            words = load_words(p, r, t0 + LG_CHUNK);
+        }
+        // ---- the listed tokens: those without a bias from the list, the others from the bias list
+        if constexpr (COUNT) {
+            __syncthreads();
+            if (tid == 0) n_listed[~chunk & 1] = 0;
+            auto settle = [&](int t, uint32_t c, float s) {
+                const float v = constrained<SHORT>(p, r, row, t, c, s);
+                if (v > best.v || (v == best.v && best.token >= 0 && t < best.token)) best = Best{v, t};
+                if (r.dst) r.dst[t] = v;
+            };
+            const int listed = n_listed[chunk & 1];
+            for (int q = tid; q < listed; q += LG_THREADS) {
+                const int i = t0 + list[q];
+                const uint32_t c = K::get(counts, i - c0);
+                if (!(c & K::BIASED)) settle(token_at(p, i), c, 0.0f);
+            }
+            for (int e = r.b0 + tid; e < r.b1; e += LG_THREADS) {
+                const int tok = p.bias_tokens[e], i = place_of(p, tok);
+                if (i < t0 || i >= t0 + LG_CHUNK) continue;
+                const uint32_t c = K::get(counts, i - c0);
+                float s = p.bias_values[e];
+                if (c & K::AGAIN) {  // the token's first entry adds up all of them, in order
+                    int f = r.b0;
+                    while (f < e && p.bias_tokens[f] != tok) f++;
+                    if (f < e) continue;
+                    for (f = e + 1; f < r.b1; f++)
+                        if (p.bias_tokens[f] == tok) s = __fadd_rn(s, p.bias_values[f]);
+                }
+                settle(tok, c, s);
+            }
+            if (more) __syncthreads();  // the next stream reuses the list
+        }
+    }
+    return best;
+}
+
 // VEC: rows are 16-byte aligned (4 consecutive tokens per load); else one token per load, the warp's consecutive.
 // COUNT: the call has histories or biases.
 template <bool VEC, bool COUNT>
-__global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsParams p) {
-    extern __shared__ __align__(16) uint32_t counts[];  // [piece], with COUNT
+__global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParams p) {
+    extern __shared__ __align__(16) uint32_t counts[];  // p.count_bytes, then the list
     __shared__ Best warp_best[LG_THREADS / 32];
-    __shared__ Best cta_best;
+    __shared__ __align__(8) Best candidate[LG_CLUSTER];  // in the first CTA: every CTA's
+    __shared__ __align__(8) uint64_t pushed;
+    __shared__ int n_listed[2];
+    const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x, row = blockIdx.y;
+    const bool push = p.choice && C > 1;
+    if (COUNT) {
+        for (int i = tid; i < p.count_bytes / 16; i += LG_THREADS) reinterpret_cast<uint4 *>(counts)[i] = uint4{0, 0, 0, 0};
+        if (tid < 2) n_listed[tid] = 0;
+    }
+    if (push) {  // the barrier for the candidates, set up before any CTA can arrive on it
+        if (rank == 0 && tid == 0) {
+            mbar_init(&pushed, (uint32_t)(C - 1));
+            fence_barrier_init();
+        }
+        __syncwarp();
+        cluster_arrive();
+    }
     grid_dependency_wait();
     grid_dependents_launch();
-    constexpr int W = VEC ? 4 : 1;                 // tokens per load
-    constexpr int STEP = LG_THREADS * W;           // tokens between a thread's loads
-    constexpr int LOADS = LG_PER_THREAD / W;
-    const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x, row = blockIdx.y;
-    const float *src = p.logits + (long long)row * p.logits_stride;
-    float *dst = p.out ? p.out + (long long)row * p.out_stride : nullptr;
-    const int v0 = min(p.vocab, rank * p.per_cta), v1 = min(p.vocab, v0 + p.per_cta);
-    const bool report = rank == 0 && tid == 0;
 
-    int h0 = 0, h1 = 0, prompt_end = 0, b0 = 0, b1 = 0;
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    if constexpr (COUNT) {
-        if (p.tokens) {
-            list_range(p.token_offsets, row, p.n_tokens, p.err, report, h0, h1);
-            const int prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
-            prompt_end = h0 + min(max(prompt, 0), h1 - h0);
-            if (p.repetition) rep = p.repetition[row];
-            if (p.frequency) freq = p.frequency[row];
-            if (p.presence) pres = p.presence[row];
-        }
-        if (p.bias_tokens) list_range(p.bias_offsets, row, p.n_bias, p.err, report, b0, b1);
-    }
-    const uint32_t *mask = nullptr;
-    bool barred = false;  // a bad mask row index allows nothing
+    // the first logits are under way before anything waits for the lists' offsets
+    Row r{};
+    r.src = p.logits + (long long)row * p.logits_stride;
+    r.dst = p.out ? p.out + (long long)row * p.out_stride : nullptr;
+    float x[LG_LOADS][4];
+    load_chunk<VEC>(p, r.src, 0, x);
+    const bool report = rank == 0 && tid == 0;
     if (p.mask) {
         const int m = p.mask_rows ? p.mask_rows[row] : row;
-        barred = m < -1 || m >= p.n_mask_rows;
-        if (barred && report) record_error(p.err, DEVERR_BADLEN);
-        if (m >= 0 && !barred) mask = p.mask + (long long)m * p.mask_stride;
+        r.barred = m < -1 || m >= p.n_mask_rows;
+        if (r.barred && report) record_error(p.err, DEVERR_BADLEN);
+        if (m >= 0 && !r.barred) r.mask = p.mask + (long long)m * p.mask_stride;
     }
-
-    Best best{-INFINITY, -1};
-    for (int t0 = v0; t0 < v1; t0 += LG_PIECE) {
-        const int n = min(LG_PIECE, v1 - t0);
-        float x[LOADS][W];
-#pragma unroll
-        for (int k = 0; k < LOADS; k++) {
-            const int i = tid * W + k * STEP;
-            if constexpr (VEC) {
-                if (i + W <= n) {
-                    const float4 f = *reinterpret_cast<const float4 *>(src + t0 + i);
-                    x[k][0] = f.x; x[k][1] = f.y; x[k][2] = f.z; x[k][3] = f.w;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < W; j++) x[k][j] = i + j < n ? src[t0 + i + j] : 0.0f;
-                }
-            } else {
-                x[k][0] = i < n ? src[t0 + i] : 0.0f;
-            }
-        }
-        if constexpr (COUNT) {
-            for (int i = tid * 4; i < n; i += LG_THREADS * 4) *reinterpret_cast<uint4 *>(counts + i) = uint4{0, 0, 0, 0};
-            __syncthreads();
-            for (int i = h0 + tid; i < h1; i += LG_THREADS) {
-                const unsigned t = (unsigned)p.tokens[i] - (unsigned)t0;
-                if (t >= (unsigned)n) continue;
-                if (i < prompt_end) atomicOr(&counts[t], LG_SEEN);
-                else atomicAdd(&counts[t], 1u);
-            }
-            for (int i = b0 + tid; i < b1; i += LG_THREADS) {
-                const unsigned t = (unsigned)p.bias_tokens[i] - (unsigned)t0;
-                if (t < (unsigned)n) atomicOr(&counts[t], LG_BIASED);
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int k = 0; k < LOADS; k++) {
-            const int i = tid * W + k * STEP;
-            if (i >= n) break;
-            const uint32_t allowed = barred ? 0u : mask ? mask[(t0 + i) >> 5] >> ((t0 + i) & 31) : 0xFFFFFFFFu;
-            uint32_t c[W] = {};
-            if constexpr (COUNT) {
-                if constexpr (VEC) {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(counts + i);
-                    c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
-                } else {
-                    c[0] = counts[i];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < W; j++) {
-                float v = x[k][j];
-                if (COUNT && c[j]) {
-                    const uint32_t made = c[j] & LG_COUNT;
-                    if (p.repetition && (c[j] & (LG_SEEN | LG_COUNT))) v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-                    if (made) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, __uint2float_rn(made))), pres);
-                    if (c[j] & LG_BIASED) {
-                        float s = 0.0f;
-                        for (int q = b0; q < b1; q++)
-                            if (p.bias_tokens[q] == t0 + i + j) s = __fadd_rn(s, p.bias_values[q]);
-                        v = __fadd_rn(v, s);
-                    }
-                }
-                if (!((allowed >> j) & 1u)) v = -INFINITY;
-                if (i + j < n && v > best.v) best = Best{v, t0 + i + j};
-                x[k][j] = v;
-            }
-            if (dst) {
-                if constexpr (VEC) {
-                    if (i + W <= n) {
-                        *reinterpret_cast<float4 *>(dst + t0 + i) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < W; j++)
-                            if (i + j < n) dst[t0 + i + j] = x[k][j];
-                    }
-                } else {
-                    dst[t0 + i] = x[k][0];
-                }
-            }
-        }
-        if (COUNT && t0 + LG_PIECE < v1) __syncthreads();  // the next piece clears the counts
+    if (COUNT && p.tokens) {
+        const int prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
+        list_range(p.token_offsets, row, p.n_tokens, p.err, report, r.h0, r.h1);
+        r.prompt_end = r.h0 + min(max(prompt, 0), r.h1 - r.h0);
     }
+    if (COUNT && p.bias_tokens) list_range(p.bias_offsets, row, p.n_bias, p.err, report, r.b0, r.b1);
+    uint16_t *list = reinterpret_cast<uint16_t *>(reinterpret_cast<uint8_t *>(counts) + p.count_bytes);
+    Best best;
+    if (!COUNT || r.h1 - r.h0 <= LG_SHORT)
+        best = work_row<VEC, COUNT, true>(p, r, row, p.count_bytes / 2, counts, list, n_listed, x);
+    else
+        best = work_row<VEC, COUNT, false>(p, r, row, p.count_bytes / 4, counts, list, n_listed, x);
 
-    // ---- the greedy choice (the same branch for every CTA of the cluster)
+    // ---- the greedy choice
     if (!p.choice) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.token, o)});
     if ((tid & 31) == 0) warp_best[tid >> 5] = best;
     __syncthreads();
-    if (tid < 32) {
-        best = tid < LG_THREADS / 32 ? warp_best[tid] : Best{-INFINITY, -1};
+    if (push) cluster_wait();  // the first CTA's barrier is set up
+    if (tid >= 32) return;
+    best = tid < LG_THREADS / 32 ? warp_best[tid] : Best{-INFINITY, -1};
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.token, o)});
-        if (tid == 0) cta_best = best;
-    }
-    if (C == 1) {
-        if (tid == 0) p.choice[row] = best.token;
+    for (int o = LG_THREADS / 64; o > 0; o >>= 1)
+        best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.token, o)});
+    if (C > 1 && rank != 0) {
+        if (tid == 0) {
+            st_cluster_u32x2(cluster_map(&candidate[rank], 0), __float_as_uint(best.v), (uint32_t)best.token);
+            mbar_arrive_remote(cluster_map(&pushed, 0));
+        }
         return;
     }
-    __syncwarp();
-    cluster_sync_all();
-    if (rank == 0 && tid == 0) {
-        for (int r = 1; r < C; r++) {
-            const uint32_t a = cluster_map(&cta_best, (uint32_t)r);
-            best = better(best, Best{ld_cluster_f32(a), (int)ld_cluster_u32(a + 4)});
-        }
-        p.choice[row] = best.token;
+    if (C > 1) {
+        // 1 s: the other CTAs of the cluster are resident and only stream their ranges
+        const bool ok = mbar_wait_cluster_bounded(&pushed, 0, 1000000000ull, p.err);
+        if (!__all_sync(0xffffffffu, ok)) return;
+        if (tid > 0) best = tid < C ? candidate[tid] : Best{-INFINITY, -1};
+#pragma unroll
+        for (int o = LG_CLUSTER / 2; o > 0; o >>= 1)
+            best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.token, o)});
     }
-    __syncwarp();
-    cluster_sync_all();  // no CTA leaves while its candidate is read
+    if (tid == 0) p.choice[row] = best.token;
 }
 
 template <bool VEC, bool COUNT>
 int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
-    const int piece = p.per_cta < LG_PIECE ? p.per_cta : LG_PIECE;
-    const size_t smem = COUNT ? (size_t)piece * sizeof(uint32_t) : 0;
-    if (COUNT) {
-        // the dynamic shared-memory opt-in is a per-device function attribute
+    const size_t smem = COUNT ? p.count_bytes + LG_CHUNK * sizeof(uint16_t) : 0;
+    {
+        // the shared-memory and cluster-size opt-ins are per-device function attributes
         static std::mutex mu;
         static bool ready[64];
         int dev = 0;
@@ -234,7 +402,9 @@ int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[dev]) {
             e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     LG_PIECE * (int)sizeof(uint32_t));
+                                     LG_COUNT_BYTES_MAX + LG_CHUNK * (int)sizeof(uint16_t));
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return fail_cuda(e, "tqk_process_logits: kernel attributes");
             ready[dev] = true;
         }
@@ -252,9 +422,9 @@ using namespace tqk;
 extern "C" int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream) {
     if (!a) return fail(TQK_EINVAL, "tqk_process_logits: NULL args");
     if (a->n_rows <= 0 || a->vocab_size <= 0) return fail(TQK_EINVAL, "tqk_process_logits: non-positive shape");
-    // token indexes and counts are 30 bits (a word per token also carries two flags)
-    if (a->vocab_size > (int)LG_COUNT || a->n_tokens > (int)LG_COUNT)
-        return fail(TQK_EUNSUPPORTED, "tqk_process_logits: vocab_size or n_tokens above 2^30 - 1");
+    // counts are 29 bits (a token's counter also carries three flags)
+    if (a->vocab_size > LG_COUNT_MAX || a->n_tokens > LG_COUNT_MAX)
+        return fail(TQK_EUNSUPPORTED, "tqk_process_logits: vocab_size or n_tokens above 2^29 - 1");
     if (a->n_rows > 65535) return fail(TQK_EINVAL, "tqk_process_logits: n_rows > 65535");
     if (!a->logits || (!a->out && !a->choice))
         return fail(TQK_EINVAL, "tqk_process_logits: NULL logits, or neither out nor choice");
@@ -306,13 +476,18 @@ extern "C" int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream)
     p.mask_rows = a->mask_rows;
     p.n_mask_rows = a->n_mask_rows;
     p.err = device_info()->err_word;
-    // CTAs per row: as many as the portable cluster has while each keeps a few thousand tokens
-    int cluster = (a->vocab_size + 2047) / 2048;
-    if (cluster > LG_CLUSTER) cluster = LG_CLUSTER;
-    p.per_cta = (int)((((int64_t)a->vocab_size + cluster - 1) / cluster + 127) / 128 * 128);
+    // CTAs per row: 8, each with at least 2048 tokens, or 16 while all of them run at once (4 per SM).  128256 tokens
+    // with everything on, 16 against 8 CTAs per row: 1 row 9.4 and 14.0 us, 64 rows 39.8 and 30.3 us, 256 rows 168 and 142 us
+    const int most = (long long)a->n_rows * LG_CLUSTER <= 4LL * device_info()->sm_count ? LG_CLUSTER : 8;
+    while (1 << p.log_c < most && a->vocab_size > 2048 << p.log_c) p.log_c++;
+    const int cluster = 1 << p.log_c;
+    p.own_blocks = (int)(((int64_t)a->vocab_size + (int64_t)cluster * LG_BLOCK - 1) / ((int64_t)cluster * LG_BLOCK));
     const bool vec = ((reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.out)) & 15) == 0 &&
                      (a->n_rows == 1 || ((ls | (p.out ? os : 0)) & 3) == 0);
     const bool count = penal || a->bias_tokens;
+    // 16 bits per token of the CTA (a long history's 32 bits take two rounds), whole chunks of 32-bit counters
+    const int64_t chunk_bytes = LG_CHUNK * 4, bytes = ((int64_t)p.own_blocks * LG_BLOCK * 2 + chunk_bytes - 1) / chunk_bytes * chunk_bytes;
+    p.count_bytes = (int)(bytes < LG_COUNT_BYTES_MAX ? bytes : LG_COUNT_BYTES_MAX);
     cudaStream_t st = (cudaStream_t)stream;
     if (vec) return count ? launch_logits<true, true>(p, cluster, st) : launch_logits<true, false>(p, cluster, st);
     return count ? launch_logits<false, true>(p, cluster, st) : launch_logits<false, false>(p, cluster, st);

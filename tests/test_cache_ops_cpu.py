@@ -101,7 +101,7 @@ LOGITS = dict(logits=FAKE, out=FAKE * 2, choice=FAKE, n_rows=2, vocab_size=100, 
 @pytest.mark.parametrize("change,status", [
     (dict(logits=None), "EINVAL"), (dict(out=None, choice=None), "EINVAL"), (dict(n_rows=0), "EINVAL"),
     (dict(vocab_size=0), "EINVAL"), (dict(n_rows=70000, n_mask_rows=70000), "EINVAL"),
-    (dict(vocab_size=2 ** 30), "EUNSUPPORTED"), (dict(n_tokens=2 ** 30), "EUNSUPPORTED"),
+    (dict(vocab_size=2 ** 29), "EUNSUPPORTED"), (dict(n_tokens=2 ** 29), "EUNSUPPORTED"),
     (dict(logits_stride=99), "EINVAL"), (dict(out_stride=99), "EINVAL"), (dict(out=FAKE, out_stride=101), "EINVAL"),
     (dict(tokens=None), "EINVAL"), (dict(token_offsets=None), "EINVAL"), (dict(n_tokens=-1), "EINVAL"),
     (dict(bias_values=None), "EINVAL"), (dict(bias_offsets=None), "EINVAL"), (dict(bias_tokens=None), "EINVAL"),
