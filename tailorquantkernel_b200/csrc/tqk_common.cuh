@@ -379,6 +379,21 @@ __device__ __forceinline__ void bulk_copy_g2s(void *dst_smem, const void *src_gm
         : "memory");
 }
 
+// The same with an L2 eviction policy (l2_evict_first): for data that is read once beside data that should stay.
+__device__ __forceinline__ uint64_t l2_evict_first() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void bulk_copy_g2s_hint(void *dst_smem, const void *src_gmem, uint32_t bytes, uint64_t *bar,
+                                                   uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+            smem_u32(dst_smem)),
+        "l"(src_gmem), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
+}
+
 // Barrier over the first NT threads of the CTA (named barrier BAR; 0 = all).
 template <int BAR, int NT>
 __device__ __forceinline__ void cta_sync() {

@@ -98,6 +98,13 @@ struct DecodeParams {
     long long score_stride;
     float2 *ml;
     int len_cap;
+    const float *weight;         // running sums [n_kv][max_tokens] of item 0, before and after the call
+    float *weight_out;
+    long long stat_stride;       // elements between items' sums (and positions)
+    int *position;
+    const int *new_pos;
+    int new_pos0;
+    int fuse_weights;            // the CTA that holds a unit's whole softmax adds its weights itself: no weight pass
 };
 
 // What a kernel hands to the weight pass of tqk_decode_q8_weights: nothing, scores and maxima in natural
@@ -108,6 +115,40 @@ enum : int { WT_NONE = 0, WT_NAT = 1, WT_LOG2 = 2 };
 // Where q head qh's scores of `item` start.
 __device__ __forceinline__ float *score_row_of(const DecodeParams &p, int item, int qh) {
     return p.scores + ((long long)item * (p.n_kv * p.group) + qh) * p.score_stride;
+}
+// A bulk copy of the K / V stream.  With scores to keep, the rows (read once per call) are the first to leave L2, so
+// that the scores are still there for the weight pass.
+template <int WT>
+__device__ __forceinline__ void stream_g2s(void *dst_smem, const void *src_gmem, uint32_t bytes, uint64_t *bar) {
+    if constexpr (WT != WT_NONE) bulk_copy_g2s_hint(dst_smem, src_gmem, bytes, bar, l2_evict_first());
+    else bulk_copy_g2s(dst_smem, src_gmem, bytes, bar);
+}
+// The sums of kv head kvh, added by a CTA that has just finished the head's whole softmax (fuse_weights): m, l are its
+// `group` q heads' final maximum and sum, the scores are the CTA's own.
+template <int WT, int BAR, int NT>
+__device__ __forceinline__ void add_weights(const DecodeParams &p, int tid, int item, int kvh, int len, const float *m,
+                                            const float *l) {
+    cta_sync<BAR, NT>();  // every thread's scores, and m and l, are visible
+    const float *src = score_row_of(p, item, kvh * p.group);
+    const long long at = (long long)item * p.stat_stride + (long long)kvh * p.max_tokens;
+    for (int t = tid; t < len; t += NT) {
+        const bool fresh = p.k_new && t == len - 1;
+        const float old = fresh ? 0.0f : p.weight[at + t];
+        float w = 0.0f;
+        for (int g0 = 0; g0 < p.group; g0 += 8) {  // 8 heads' loads in flight
+            float s[8];
+#pragma unroll
+            for (int g = 0; g < 8; g++) s[g] = g0 + g < p.group ? __ldcg(src + (g0 + g) * p.score_stride + t) : 0.0f;
+#pragma unroll
+            for (int g = 0; g < 8; g++) {
+                if (g0 + g >= p.group) break;
+                const float d = s[g] - m[g0 + g];
+                w = fmaf(WT == WT_LOG2 ? ex2f(d) : expf(d), __fdiv_rn(1.0f, l[g0 + g]), w);
+            }
+        }
+        p.weight_out[at + t] = old + w;
+        if (fresh && p.position) p.position[at + t] = p.new_pos ? p.new_pos[item] : p.new_pos0;
+    }
 }
 // Clamped length of an item; records lengths outside [0, cap].
 __device__ __forceinline__ int clamp_len(const DecodeParams &p, int len, int cap, bool report) {
@@ -727,6 +768,7 @@ __global__ void __launch_bounds__(DEC_THREADS) decode_q8_kernel(const DecodePara
     };
     finish_split<HD, GMAX, DEC_THREADS, 0, WT>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, m_s, l_s,
                                               red + DEC_WARPS * GMAX * HD, flag);
+    if (WT != WT_NONE && p.fuse_weights) add_weights<WT, 0, DEC_THREADS>(p, tid, item, kvh, len, m_s, l_s);
 }
 
 }  // namespace tqk
@@ -1255,6 +1297,11 @@ int decode_impl(const tqk_decode_args *a, const tqk_gather_dst *gd, void *worksp
     return dispatch(pl, p, grid, st, nullptr);
 }
 
+// Lengths up to which an unsplit call adds its weights in the decode itself.  A second launch costs the smallest calls
+// more than it does (14 q heads at 3 tokens: 9.0 us with it, 7.4 us without; 64 sequences of 64 tokens 10.8 and 10.1 us);
+// from a few hundred tokens on its wider grid wins (64 sequences of 500 tokens: 21.8 us with it, 25.7 us without).
+constexpr int FUSE_WEIGHTS_LEN = 64;
+
 // Workspace of tqk_decode_q8_weights: the decode's tickets (always the whole region, so that the scores of
 // a call without splits do not touch the tickets of the calls it shares the workspace with) and partials,
 // then every q head's scores and final (max, sum).
@@ -1341,31 +1388,21 @@ extern "C" int tqk_decode_q8_weights(const tqk_decode_args *a, const tqk_weights
     p.score_stride = ws.score_stride;
     p.ml = reinterpret_cast<float2 *>(base + ws.ml_off);
     p.len_cap = pl.max_len;
+    p.weight = w->weight;
+    p.weight_out = w->weight_out;
+    p.stat_stride = w->item_stride;
+    p.position = w->position;
+    p.new_pos = w->new_pos;
+    p.new_pos0 = w->new_pos0;
+    // one CTA holds the whole softmax of a head and has few scores to read back
+    p.fuse_weights = !pl.balanced && pl.max_splits == 1 && pl.head_slices == 1 && pl.max_len <= FUSE_WEIGHTS_LEN;
     rc = pl.balanced ? dispatch(pl, p, dim3((unsigned)pl.bal_ctas), st, nullptr, true)
                      : dispatch(pl, p, dim3((unsigned)pl.max_splits, (unsigned)pl.pairs, (unsigned)a->n_items), st, nullptr);
-    if (rc || pl.max_len == 0) return rc;  // nothing cached anywhere: no weights
-    WeightParams q{};
-    q.scores = p.scores;
-    q.score_stride = p.score_stride;
-    q.ml = p.ml;
-    q.group = p.group;
-    q.n_kv = p.n_kv;
-    q.max_tokens = p.max_tokens;
-    q.len_cap = p.len_cap;
-    q.lens = p.lens;
-    q.len0 = p.len0;
-    q.len_step = p.len_step;
-    q.weight = w->weight;
-    q.weight_out = w->weight_out;
-    q.item_stride = w->item_stride;
-    q.appended = a->k_new != nullptr;
-    q.position = w->position;
-    q.new_pos = w->new_pos;
-    q.new_pos0 = w->new_pos0;
+    if (rc || p.fuse_weights || pl.max_len == 0) return rc;
     const int per = WP_THREADS * WP_TOKENS;
     const dim3 grid((unsigned)((pl.max_len + per - 1) / per), (unsigned)a->n_kv_heads, (unsigned)a->n_items);
-    return pl.mma ? launch_pdl(weight_sum_kernel<WT_LOG2>, grid, dim3(WP_THREADS), 0, st, q)
-                  : launch_pdl(weight_sum_kernel<WT_NAT>, grid, dim3(WP_THREADS), 0, st, q);
+    return pl.mma ? launch_pdl(weight_sum_kernel<WT_LOG2>, grid, dim3(WP_THREADS), 0, st, p)
+                  : launch_pdl(weight_sum_kernel<WT_NAT>, grid, dim3(WP_THREADS), 0, st, p);
 }
 
 extern "C" int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t workspace_bytes,

@@ -441,8 +441,8 @@ __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const Decode
         const uint32_t bytes = (uint32_t)(rows * ROW);
         uint8_t *ks = smem + slot * L::STAGE_BYTES;
         mbar_arrive_expect_tx(&full[slot], 2 * bytes);
-        bulk_copy_g2s(ks, kbase + (long long)t0 * ROW, bytes, &full[slot]);
-        bulk_copy_g2s(ks + L::TILE, vbase + (long long)t0 * ROW, bytes, &full[slot]);
+        stream_g2s<WT>(ks, kbase + (long long)t0 * ROW, bytes, &full[slot]);
+        stream_g2s<WT>(ks + L::TILE, vbase + (long long)t0 * ROW, bytes, &full[slot]);
     };
 
     const int producer = MMA_WARPS * 32;
@@ -628,6 +628,7 @@ __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const Decode
     };
     finish_split<HD, GPAD, MMA_WARPS * 32, 1, WT>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, fm, fl,
                                                   wts, flag);
+    if (WT != WT_NONE && p.fuse_weights) add_weights<WT, 1, MMA_WARPS * 32>(p, tid, item, kvh, len, fm, fl);
 }
 
 }  // namespace tqk

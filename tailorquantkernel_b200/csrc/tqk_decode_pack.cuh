@@ -626,10 +626,10 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
         uint8_t *st = smem + slot * L::STAGE_BYTES;
         const long long o = (long long)t0 * ROW;
         mbar_arrive_expect_tx(&full[slot], 4 * bytes);
-        bulk_copy_g2s(st, ka + o, bytes, &full[slot]);
-        bulk_copy_g2s(st + L::PLANE, ka + head_bytes + o, bytes, &full[slot]);
-        bulk_copy_g2s(st + 2 * L::PLANE, va + o, bytes, &full[slot]);
-        bulk_copy_g2s(st + 3 * L::PLANE, va + head_bytes + o, bytes, &full[slot]);
+        stream_g2s<WT>(st, ka + o, bytes, &full[slot]);
+        stream_g2s<WT>(st + L::PLANE, ka + head_bytes + o, bytes, &full[slot]);
+        stream_g2s<WT>(st + 2 * L::PLANE, va + o, bytes, &full[slot]);
+        stream_g2s<WT>(st + 3 * L::PLANE, va + head_bytes + o, bytes, &full[slot]);
     };
 
     const int producer = PK_WARPS * 32;
@@ -719,6 +719,10 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
     auto acc_of = [&](int gg, int c) { return r.acc<L::RED_STRIDE>(gg, c); };
     finish_split<HD, 8, PK_WARPS * 32, 1, WT>(p, tid, item, pair, s, n_splits, qh0, G, out_item, acc_of, r.fm(),
                                               r.fl(), wts, flag);
+    if (WT != WT_NONE && p.fuse_weights) {
+        add_weights<WT, 1, PK_WARPS * 32>(p, tid, item, kvh_a, len, r.fm(), r.fl());
+        add_weights<WT, 1, PK_WARPS * 32>(p, tid, item, kvh_a + 1, len, r.fm() + 4, r.fl() + 4);
+    }
 }
 
 
@@ -894,10 +898,10 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
                 uint8_t *stg = smem + slot * L::STAGE_BYTES;
                 const long long o = (long long)t0 * ROW;
                 mbar_arrive_expect_tx(&full[slot], 4 * bytes);
-                bulk_copy_g2s(stg, ka + o, bytes, &full[slot]);
-                bulk_copy_g2s(stg + L::PLANE, ka + head_bytes + o, bytes, &full[slot]);
-                bulk_copy_g2s(stg + 2 * L::PLANE, va + o, bytes, &full[slot]);
-                bulk_copy_g2s(stg + 3 * L::PLANE, va + head_bytes + o, bytes, &full[slot]);
+                stream_g2s<WT>(stg, ka + o, bytes, &full[slot]);
+                stream_g2s<WT>(stg + L::PLANE, ka + head_bytes + o, bytes, &full[slot]);
+                stream_g2s<WT>(stg + 2 * L::PLANE, va + o, bytes, &full[slot]);
+                stream_g2s<WT>(stg + 3 * L::PLANE, va + head_bytes + o, bytes, &full[slot]);
             }
             g = sg.ubase + sg.lt1;
         }
