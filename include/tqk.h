@@ -222,8 +222,9 @@ TQK_API int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t work
  *     q head and position: tqk_decode_weights_workspace_size() bytes, under
  *     tqk_decode_q8's rules (zeroed once, ordered on one stream, shared with
  *     tqk_decode_q8 if large enough); NULL = library-owned, per (device, stream).
- *   - Two launches, capturable in a CUDA graph (with a caller workspace, or after
- *     one earlier call on the same stream outside capture). */
+ *   - One or two launches.  Under stream capture a caller workspace is required
+ *     (TQK_EWORKSPACE otherwise): graphs that may run at the same time need one
+ *     each. */
 typedef struct {
     const float *weight;         /* device, [n_kv][max_tokens] of item 0: the sums before the call */
     float *weight_out;           /* device, same layout: the sums after it; may be weight (the usual case), else

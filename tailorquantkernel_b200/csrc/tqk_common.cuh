@@ -394,6 +394,30 @@ __device__ __forceinline__ void bulk_copy_g2s_hint(void *dst_smem, const void *s
         : "memory");
 }
 
+// Loads of data that is used once: no line is kept in L1.
+__device__ __forceinline__ float4 load_stream(const float4 *p) {
+    float4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "l"(p)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_stream(const float *p) {
+    float v;
+    asm volatile("ld.global.L1::no_allocate.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+
+// 4- and 16-byte asynchronous copies global -> shared, and the wait for all of this thread's.
+__device__ __forceinline__ void copy_async_4(void *dst_smem, const void *src_gmem) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst_smem)), "l"(src_gmem) : "memory");
+}
+__device__ __forceinline__ void copy_async_16(void *dst_smem, const void *src_gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst_smem)), "l"(src_gmem) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Barrier over the first NT threads of the CTA (named barrier BAR; 0 = all).
 template <int BAR, int NT>
 __device__ __forceinline__ void cta_sync() {

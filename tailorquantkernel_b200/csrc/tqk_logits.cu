@@ -10,12 +10,12 @@
 //   * while the first logits are on their way, every CTA scans the history and
 //     counts its own tokens in shared memory (a counter per token: seen, in the
 //     bias list, and the count after the prompt; integer atomics, so their order
-//     does not show).  Frequent tokens have neighbouring ids in many vocabularies;
-//     dealing out small blocks spreads them over the CTAs;
-//   * the stream leaves counted tokens alone and puts them on a list; the list is
-//     worked off with full warps, so the division and the branches of the
-//     penalties cost by the distinct tokens of the history, not by the vocabulary;
-//     the next logits are loaded meanwhile;
+//     does not show) and marks them in a bitmap.  Frequent tokens have neighbouring
+//     ids in many vocabularies; dealing out small blocks spreads them over the CTAs;
+//   * the stream reads the bitmap like a second mask; each warp then lists its
+//     marked tokens and works the list off with all lanes, so the division and the
+//     branches of the penalties cost by the distinct tokens of the history, not by
+//     the vocabulary;
 //   * each CTA pushes its candidate for the greedy choice to the first CTA's
 //     shared memory and leaves.
 #include "tqk_internal.h"
@@ -33,24 +33,27 @@ constexpr int LG_LOADS = 8;                              // blocks per warp and 
 constexpr int LG_CHUNK = LG_WARPS * LG_LOADS * LG_BLOCK; // 8192 tokens
 constexpr int LG_CLUSTER = 16;                           // most CTAs per row (non-portable above 8), a power of two
 constexpr int LG_COUNT_BYTES_MAX = 64 << 10;             // counters per CTA
-constexpr int LG_SCAN = 8;                               // history entries in flight per thread
-
-// Counters: 16 bits per token (two to a word) for histories of up to LG_SHORT entries, else 32 bits.  From the top:
-// seen, in the bias list, more than once in the bias list, and the count after the prompt.
+constexpr int LG_LIST = 256;                             // listed tokens per warp at a time
+constexpr int LG_STAGE = LG_WARPS * LG_LIST;             // history entries staged at a time, beside the lists
+constexpr int LG_SCAN = LG_STAGE / LG_THREADS / 4;       // ... 16-byte copies per thread
+// Counters: 16 bits per token (two to a word) for histories with up to LG_SHORT entries behind the prompt, else 32 bits.
+// From the top: seen, in the bias list, more than once in the bias list, and the count after the prompt.  The width is
+// a value of the row, not of the type: two copies of the row's work in one kernel miss the instruction cache (256 rows
+// of 128256 tokens: 75 us with both, 67 us with one).
 constexpr int LG_SHORT = (1 << 13) - 1;
-template <bool SHORT>
-struct Counter {
-    static constexpr int BITS = SHORT ? 16 : 32;
-    static constexpr uint32_t SEEN = 1u << (BITS - 1), BIASED = 1u << (BITS - 2), AGAIN = 1u << (BITS - 3);
-    static constexpr uint32_t COUNT = AGAIN - 1;
-    // the word of token t, and the place of its counter in it
-    static __device__ __forceinline__ int word(int t) { return SHORT ? t >> 1 : t; }
-    static __device__ __forceinline__ int shift(int t) { return SHORT ? (t & 1) * 16 : 0; }
-    static __device__ __forceinline__ uint32_t get(const uint32_t *c, int t) {
-        return SHORT ? (c[t >> 1] >> shift(t)) & 0xFFFFu : c[t];
-    }
+constexpr int LG_COUNT_MAX = (1 << 29) - 1;
+struct Counters {
+    uint32_t *words;
+    int half;  // 1: 16 bits, 0: 32 bits
+    __device__ __forceinline__ uint32_t seen() const { return half ? 0x8000u : 0x80000000u; }
+    __device__ __forceinline__ uint32_t biased() const { return seen() >> 1; }
+    __device__ __forceinline__ uint32_t again() const { return seen() >> 2; }
+    __device__ __forceinline__ uint32_t count() const { return (seen() >> 2) - 1; }
+    // the word of token t, and its counter's place in it
+    __device__ __forceinline__ uint32_t *word(int t) const { return words + (t >> half); }
+    __device__ __forceinline__ int shift(int t) const { return (t & half) * 16; }
+    __device__ __forceinline__ uint32_t get(int t) const { return (*word(t) >> shift(t)) & (seen() * 2 - 1); }
 };
-constexpr int LG_COUNT_MAX = Counter<false>::COUNT;
 
 struct LogitsParams {
     const float *logits;
@@ -95,6 +98,9 @@ __device__ __forceinline__ Best better(Best a, Best b) {
     return take ? b : a;
 }
 
+// 16-byte units of the counters and the bitmap of counted tokens behind them, a bit per 16-bit counter's token.
+__device__ __forceinline__ int zero_units(const LogitsParams &p) { return (p.count_bytes + p.count_bytes / 16) / 16; }
+
 // What all threads of a CTA know of their row.
 struct Row {
     const float *src;
@@ -102,6 +108,9 @@ struct Row {
     const uint32_t *mask;  // or nullptr
     bool barred;           // a bad mask row index: nothing is allowed
     int h0, h1, prompt_end, b0, b1;
+    Counters counters;
+    int span;  // tokens that the counters cover at a time, whole chunks
+    float repetition, frequency, presence;
 };
 
 // Bit t of the row's mask.
@@ -109,21 +118,13 @@ __device__ __forceinline__ bool allowed_token(const Row &r, int t) {
     return !r.barred && (!r.mask || (r.mask[t >> 5] >> (t & 31)) & 1u);
 }
 
-// A listed token's final value: penalties by its counter c, then its biases' sum s.
-template <bool SHORT>
-__device__ __forceinline__ float constrained(const LogitsParams &p, const Row &r, int row, int t, uint32_t c, float s) {
-    using K = Counter<SHORT>;
-    float v = r.src[t];  // in place: still the logit
-    if (p.repetition && (c & (K::SEEN | K::COUNT))) {
-        const float rep = p.repetition[row];
-        v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-    }
-    if (c & K::COUNT) {
-        const float freq = p.frequency ? p.frequency[row] : 0.0f, pres = p.presence ? p.presence[row] : 0.0f;
-        v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, __uint2float_rn(c & K::COUNT))), pres);
-    }
-    if (c & K::BIASED) v = __fadd_rn(v, s);
-    return allowed_token(r, t) ? v : -INFINITY;
+// A listed token's final value from its logit v: penalties by its counter c, then its biases' sum s.
+__device__ __forceinline__ float constrained(const LogitsParams &p, const Row &r, float v, uint32_t c, float s) {
+    const Counters &k = r.counters;
+    if (p.repetition && (c & (k.seen() | k.count())))
+        v = v > 0.0f ? __fdiv_rn(v, r.repetition) : __fmul_rn(v, r.repetition);
+    if (c & k.count()) v = __fsub_rn(__fsub_rn(v, __fmul_rn(r.frequency, __uint2float_rn(c & k.count()))), r.presence);
+    return c & k.biased() ? __fadd_rn(v, s) : v;
 }
 
 // The CTA's tokens: block b of the row is block b >> log_c of CTA b mod C.  The row's token at place i of them:
@@ -132,31 +133,35 @@ __device__ __forceinline__ int token_at(const LogitsParams &p, int i) {
 }
 // ... and the place of token `tok`, or -1 when it is another CTA's or outside the vocabulary.
 __device__ __forceinline__ int place_of(const LogitsParams &p, int tok) {
-    const int blk = tok / LG_BLOCK;
-    if ((unsigned)tok >= (unsigned)p.vocab || (blk & ((1 << p.log_c) - 1)) != (int)blockIdx.x) return -1;
-    return (blk >> p.log_c) * LG_BLOCK + tok % LG_BLOCK;
+    const unsigned blk = (unsigned)tok / LG_BLOCK;
+    const bool own = (blk & ((1u << p.log_c) - 1)) == blockIdx.x && (unsigned)tok < (unsigned)p.vocab;
+    return own ? (int)(blk >> p.log_c) * LG_BLOCK + tok % LG_BLOCK : -1;
 }
 
 // The logits of the chunk at place t0, 8 blocks per warp.  VEC: tokens 4 lane .. 4 lane + 3 of each block; else tokens
-// lane, 32 + lane, 64 + lane, 96 + lane.
+// lane, 32 + lane, 64 + lane, 96 + lane.  Places behind the vocabulary hold 0.
 template <bool VEC>
 __device__ __forceinline__ void load_chunk(const LogitsParams &p, const float *src, int t0, float (&x)[LG_LOADS][4]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int first0 = token_at(p, t0 + warp * LG_BLOCK), step = (LG_WARPS << p.log_c) * LG_BLOCK;
+    const float *at = src + first0 + (VEC ? 4 * lane : lane);
 #pragma unroll
-    for (int k = 0; k < LG_LOADS; k++) {
-        const int first = token_at(p, t0 + (warp + k * LG_WARPS) * LG_BLOCK);
-        if constexpr (VEC) {
-            const int t = first + 4 * lane;
-            if (t + 4 <= p.vocab) {
-                const float4 f = *reinterpret_cast<const float4 *>(src + t);
+    for (int k = 0; k < LG_LOADS; k++, at += step) {
+        const int left = p.vocab - first0 - k * step;  // tokens from the block's first on
+        if (left >= LG_BLOCK) {
+            if constexpr (VEC) {
+                const float4 f = load_stream(reinterpret_cast<const float4 *>(at));
                 x[k][0] = f.x; x[k][1] = f.y; x[k][2] = f.z; x[k][3] = f.w;
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[k][j] = t + j < p.vocab ? src[t + j] : 0.0f;
+                for (int j = 0; j < 4; j++) x[k][j] = load_stream(at + 32 * j);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[k][j] = first + 32 * j + lane < p.vocab ? src[first + 32 * j + lane] : 0.0f;
+            for (int j = 0; j < 4; j++) {
+                const int in = VEC ? j : 32 * j;
+                x[k][j] = in + (VEC ? 4 * lane : lane) < left ? at[in] : 0.0f;
+            }
         }
     }
 }
@@ -170,155 +175,231 @@ __device__ __forceinline__ uint32_t load_words(const LogitsParams &p, const Row 
     }
     return words;
 }
+// The bits of this lane's 4 tokens of block k, from words laid out as above.
+template <bool VEC>
+__device__ __forceinline__ uint32_t lane_bits(uint32_t words, int k) {
+    const int lane = threadIdx.x & 31;
+    if constexpr (VEC) return (__shfl_sync(0xffffffffu, words, 4 * k + (lane >> 3)) >> (4 * (lane & 7))) & 0xFu;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) bits |= ((__shfl_sync(0xffffffffu, words, 4 * k + j) >> lane) & 1u) << j;
+    return bits;
+}
 
-// This CTA's share of a row.  On entry x holds the first chunk, and the counters, which cover `span` tokens (whole
-// chunks) at a time, and both list lengths are zero.
-template <bool VEC, bool COUNT, bool SHORT>
-__device__ __forceinline__ Best work_row(const LogitsParams &p, const Row &r, int row, int span, uint32_t *counts,
-                                         uint16_t *list, int *n_listed, float (&x)[LG_LOADS][4]) {
-    using K = Counter<SHORT>;
+// Counts the history's entries among this CTA's tokens [c0, c0 + span) and marks them in the bitmap.  The entries are
+// staged in shared memory, 2048 at a time, so that they take no registers beside the logits; each warp picks the
+// CTA's (one in C) out of its 256 and then counts those with all lanes.
+__device__ __forceinline__ void count_history(const LogitsParams &p, const Row &r, int c0, uint32_t *bitmap, uint32_t *lists) {
+    const Counters &k = r.counters;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int own = p.own_blocks * LG_BLOCK;
-    Best best{-INFINITY, -1};
-    uint32_t words = load_words(p, r, 0);
-    for (int t0 = 0, c0 = 0, chunk = 0; t0 < own; t0 += LG_CHUNK, chunk++) {
-        if constexpr (COUNT) {
-            if (t0 == 0 || t0 == c0 + span) {
-                // ---- the counters of the tokens from t0 on
-                if (t0 > 0) {  // the last span's are done with (the barrier after its last list)
-                    for (int i = tid; i < p.count_bytes / 16; i += LG_THREADS)
-                        reinterpret_cast<uint4 *>(counts)[i] = uint4{0, 0, 0, 0};
-                }
-                c0 = t0;
-                __syncthreads();
-                for (int i0 = r.h0 + tid; i0 < r.h1; i0 += LG_SCAN * LG_THREADS) {
-                    int tok[LG_SCAN];
+    uint32_t *staged = lists + LG_WARPS * LG_LIST, *picked = lists + warp * LG_LIST;  // tokens, bit 31: generated
+    const uint32_t below = (1u << lane) - 1, deal = (1u << p.log_c) - 1;
+    // from a 16-byte boundary on; entries before h0 are skipped.  An array that is not 16-byte aligned is copied word by word
+    const bool wide = (reinterpret_cast<uintptr_t>(p.tokens) & 15) == 0;
+#pragma unroll 1
+    for (int base = r.h0 & ~3; base < r.h1; base += LG_STAGE) {
 #pragma unroll
-                    for (int q = 0; q < LG_SCAN; q++) {
-                        const int i = i0 + q * LG_THREADS;
-                        tok[q] = i < r.h1 ? p.tokens[i] : -1;
-                    }
-#pragma unroll
-                    for (int q = 0; q < LG_SCAN; q++) {
-                        const int t = place_of(p, tok[q]) - c0;
-                        if ((unsigned)t >= (unsigned)span) continue;
-                        if (i0 + q * LG_THREADS < r.prompt_end) atomicOr(&counts[K::word(t)], K::SEEN << K::shift(t));
-                        else atomicAdd(&counts[K::word(t)], 1u << K::shift(t));
-                    }
-                }
-                for (int i = r.b0 + tid; i < r.b1; i += LG_THREADS) {
-                    const int t = place_of(p, p.bias_tokens[i]) - c0;
-                    if ((unsigned)t >= (unsigned)span) continue;
-                    const uint32_t flag = K::BIASED << K::shift(t);
-                    if (atomicOr(&counts[K::word(t)], flag) & flag) atomicOr(&counts[K::word(t)], K::AGAIN << K::shift(t));
-                }
-                __syncthreads();
-            }
-        }
-        // ---- the stream: counted tokens keep their logit for now
-#pragma unroll
-        for (int k = 0; k < LG_LOADS; k++) {
-            const int i = (warp + k * LG_WARPS) * LG_BLOCK;  // the block's place in the chunk
-            const int first = token_at(p, t0 + i);
-            uint32_t bits = 0;
-            if constexpr (VEC) bits = __shfl_sync(0xffffffffu, words, k * 4 + (lane >> 3)) >> (4 * (lane & 7));
-            uint32_t c[4] = {};
-            if constexpr (COUNT) {
-                const int at = t0 - c0 + i;
-                if constexpr (!VEC) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) c[j] = K::get(counts, at + 32 * j + lane);
-                } else if constexpr (SHORT) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(counts + (at + 4 * lane) / 2);
-                    c[0] = u.x & 0xFFFFu; c[1] = u.x >> 16; c[2] = u.y & 0xFFFFu; c[3] = u.y >> 16;
-                } else {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(counts + at + 4 * lane);
-                    c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int in = VEC ? 4 * lane + j : 32 * j + lane;
-                bool allowed;
-                if constexpr (VEC) allowed = (bits >> j) & 1u;
-                else allowed = (__shfl_sync(0xffffffffu, words, k * 4 + j) >> lane) & 1u;
-                if (COUNT && c[j]) {
-                    list[atomicAdd(&n_listed[chunk & 1], 1)] = (uint16_t)(i + in);
-                } else {
-                    if (!allowed) x[k][j] = -INFINITY;
-                    if (x[k][j] > best.v && first + in < p.vocab) best = Best{x[k][j], first + in};
-                }
-            }
-            if (!r.dst) continue;
-            if constexpr (VEC) {
-                const int t = first + 4 * lane;
-                if (t + 4 <= p.vocab) {
-                    *reinterpret_cast<float4 *>(r.dst + t) = make_float4(x[k][0], x[k][1], x[k][2], x[k][3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (t + j < p.vocab) r.dst[t + j] = x[k][j];
-                }
+        for (int q = 0; q < LG_SCAN; q++) {
+            const int e = 4 * (q * LG_THREADS + tid), i = base + e;
+            if (wide && i + 4 <= p.n_tokens) {
+                if (i < r.h1) copy_async_16(staged + e, p.tokens + i);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (first + 32 * j + lane < p.vocab) r.dst[first + 32 * j + lane] = x[k][j];
+                    if (i + j < r.h1) copy_async_4(staged + e + j, p.tokens + i + j);
             }
         }
-        const bool more = t0 + LG_CHUNK < own;
-        if (more) {
+        copy_async_wait_all();  // each thread reads only what it copied
+        int n = 0;
+#pragma unroll
+        for (int q = 0; q < LG_SCAN; q++) {
+            const int e = 4 * (q * LG_THREADS + tid), i = base + e;
+            const uint4 v = *reinterpret_cast<const uint4 *>(staged + e);
+            const uint32_t tok[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool mine = ((tok[j] / LG_BLOCK) & deal) == blockIdx.x && tok[j] < (uint32_t)p.vocab &&
+                                  i + j >= r.h0 && i + j < r.h1;
+                const uint32_t lanes = __ballot_sync(0xffffffffu, mine);
+                if (mine) picked[n + __popc(lanes & below)] = tok[j] | (i + j >= r.prompt_end ? 0x80000000u : 0u);
+                n += __popc(lanes);
+            }
+        }
+        __syncwarp();
+        for (int q = lane; q < n; q += 32) {
+            const uint32_t e = picked[q], tok = e & 0x7FFFFFFFu;
+            const int t = (int)((tok / LG_BLOCK) >> p.log_c) * LG_BLOCK + (int)(tok % LG_BLOCK) - c0;
+            if ((unsigned)t >= (unsigned)r.span) continue;
+            // frequent tokens meet here again and again: a flag that is set already needs no atomic
+            const uint32_t flag = k.seen() << k.shift(t), bit = 1u << (t & 31);
+            if (e >> 31) atomicAdd(k.word(t), 1u << k.shift(t));
+            else if (!(*k.word(t) & flag)) atomicOr(k.word(t), flag);
+            if (!(bitmap[t >> 5] & bit)) atomicOr(&bitmap[t >> 5], bit);
+        }
+        __syncwarp();
+    }
+}
+
+// This CTA's share of a row.  On entry x holds the first chunk, and the counters and their bitmap are zero.
+template <bool VEC, bool COUNT>
+__device__ __forceinline__ Best work_row(const LogitsParams &p, const Row &r, uint32_t *bitmap, uint32_t *lists,
+                                         float (&x)[LG_LOADS][4]) {
+    const Counters &counters = r.counters;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int own = p.own_blocks * LG_BLOCK, step = (LG_WARPS << p.log_c) * LG_BLOCK;
+    Best top{-INFINITY, -1};   // of the warp's streamed tokens
+    Best best{-INFINITY, -1};  // of this thread's listed ones
+    uint16_t *list = reinterpret_cast<uint16_t *>(lists + warp * LG_LIST);  // this warp's: bits of its words, 32 w + b
+    uint32_t words = load_words(p, r, 0);
+    int c0 = 0;
+    auto settle = [&](int t, float v) {
+        if (v > best.v || (v == best.v && best.token >= 0 && t < best.token)) best = Best{v, t};
+        if (r.dst) r.dst[t] = v;
+    };
+    // the warp's marked tokens of the chunk at t0, `mask` its mask words; those with a bias are left to the bias list
+    auto work_off = [&](uint32_t marks, uint32_t mask, int t0) {
+        while (__any_sync(0xffffffffu, marks != 0)) {  // once, unless there are more than the list holds
+            int at = __popc(marks);
+            if (__reduce_add_sync(0xffffffffu, at) > LG_LIST) at = min(at, LG_LIST / 32);
+            const int n_own = at;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, at, o);
+                if (lane >= o) at += x;
+            }
+            const int n = __shfl_sync(0xffffffffu, at, 31);
+            at -= n_own;
+            for (int q = 0; q < n_own; q++, marks &= marks - 1) list[at + q] = (uint16_t)(32 * lane + __ffs(marks) - 1);
+            __syncwarp();
+            for (int q0 = 0; q0 < n; q0 += 32) {
+                const int e = q0 + lane < n ? list[q0 + lane] : 0;
+                const bool allowed = (__shfl_sync(0xffffffffu, mask, e >> 5) >> (e & 31)) & 1u;
+                if (q0 + lane >= n) continue;
+                const int i = t0 + (warp + (e >> 7) * LG_WARPS) * LG_BLOCK + e % LG_BLOCK, t = token_at(p, i);
+                const float v = __ldcg(r.src + t);  // in place: still the logit
+                const uint32_t c = counters.get(i - c0);
+                if (!(c & counters.biased())) settle(t, allowed ? constrained(p, r, v, c, 0.0f) : -INFINITY);
+            }
+            __syncwarp();
+        }
+    };
+    for (int t0 = 0; t0 < own; t0 += LG_CHUNK) {
+        if constexpr (COUNT) {
+            if (t0 == 0 || t0 == c0 + r.span) {
+                // ---- the counters of the tokens from t0 on
+                if (t0 > 0) {
+                    __syncthreads();  // the last span's are done with
+                    for (int i = tid; i < zero_units(p); i += LG_THREADS)
+                        reinterpret_cast<uint4 *>(counters.words)[i] = uint4{0, 0, 0, 0};
+                }
+                c0 = t0;
+                __syncthreads();
+                count_history(p, r, c0, bitmap, lists);
+                for (int i = r.b0 + tid; i < r.b1; i += LG_THREADS) {
+                    const int t = place_of(p, p.bias_tokens[i]) - c0;
+                    if ((unsigned)t >= (unsigned)r.span) continue;
+                    const uint32_t flag = counters.biased() << counters.shift(t);
+                    if (atomicOr(counters.word(t), flag) & flag) atomicOr(counters.word(t), flag >> 1);
+                    atomicOr(&bitmap[t >> 5], 1u << (t & 31));
+                }
+                __syncthreads();
+            }
+        }
+        // ---- the stream: marked tokens keep their logit for now
+        uint32_t marks = 0;
+        if constexpr (COUNT) marks = bitmap[(t0 - c0 + (warp + (lane >> 2) * LG_WARPS) * LG_BLOCK) / 32 + (lane & 3)];
+        const int first0 = token_at(p, t0 + warp * LG_BLOCK);
+        float *to = r.dst ? r.dst + first0 + (VEC ? 4 * lane : lane) : nullptr;
+#pragma unroll
+        for (int k = 0; k < LG_LOADS; k++) {
+            const int left = p.vocab - first0 - k * step;  // tokens from the block's first on
+            const uint32_t allowed = lane_bits<VEC>(words, k), listed = COUNT ? lane_bits<VEC>(marks, k) : 0u;
+            float y[4];  // what is stored
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = ((allowed | listed) >> j) & 1u ? x[k][j] : -INFINITY;
+            if (r.dst) {
+                float *d = to + k * step;
+                if (left >= LG_BLOCK) {
+                    if constexpr (VEC) {
+                        *reinterpret_cast<float4 *>(d) = make_float4(y[0], y[1], y[2], y[3]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) d[32 * j] = y[j];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int in = VEC ? j : 32 * j;
+                        if (in + (VEC ? 4 * lane : lane) < left) d[in] = y[j];
+                    }
+                }
+            }
+            // the warp's best: a block seldom beats all blocks before it, so one vote per block (NaN loses every
+            // comparison); when one may, the largest value's first token among those that the stream settles
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > top.v)) {
+                float most = -INFINITY;
+                unsigned token = UINT_MAX;
+#pragma unroll
+                for (int j = 3; j >= 0; j--) {
+                    const int in = VEC ? 4 * lane + j : 32 * j + lane;
+                    if (y[j] >= most && y[j] > top.v && in < left && !((listed >> j) & 1u)) {
+                        most = y[j];
+                        token = first0 + k * step + in;
+                    }
+                }
+                const int bits = __float_as_int(most + 0.0f);  // -0 as 0
+                const int order = token != UINT_MAX ? bits ^ ((bits >> 31) & 0x7FFFFFFF) : INT_MIN;
+                const int o = __reduce_max_sync(0xffffffffu, order);
+                if (o != INT_MIN) {
+                    top.v = __int_as_float(o ^ ((o >> 31) & 0x7FFFFFFF));
+                    top.token = (int)__reduce_min_sync(0xffffffffu, order == o ? token : UINT_MAX);
+                }
+            }
+        }
+        const uint32_t mask = words;
+        if (t0 + LG_CHUNK < own) {  // the next logits load while the marked tokens are worked off
             load_chunk<VEC>(p, r.src, t0 + LG_CHUNK, x);
             words = load_words(p, r, t0 + LG_CHUNK);
         }
-        // ---- the listed tokens: those without a bias from the list, the others from the bias list
         if constexpr (COUNT) {
-            __syncthreads();
-            if (tid == 0) n_listed[~chunk & 1] = 0;
-            auto settle = [&](int t, uint32_t c, float s) {
-                const float v = constrained<SHORT>(p, r, row, t, c, s);
-                if (v > best.v || (v == best.v && best.token >= 0 && t < best.token)) best = Best{v, t};
-                if (r.dst) r.dst[t] = v;
-            };
-            const int listed = n_listed[chunk & 1];
-            for (int q = tid; q < listed; q += LG_THREADS) {
-                const int i = t0 + list[q];
-                const uint32_t c = K::get(counts, i - c0);
-                if (!(c & K::BIASED)) settle(token_at(p, i), c, 0.0f);
-            }
-            for (int e = r.b0 + tid; e < r.b1; e += LG_THREADS) {
-                const int tok = p.bias_tokens[e], i = place_of(p, tok);
-                if (i < t0 || i >= t0 + LG_CHUNK) continue;
-                const uint32_t c = K::get(counts, i - c0);
-                float s = p.bias_values[e];
-                if (c & K::AGAIN) {  // the token's first entry adds up all of them, in order
-                    int f = r.b0;
-                    while (f < e && p.bias_tokens[f] != tok) f++;
-                    if (f < e) continue;
-                    for (f = e + 1; f < r.b1; f++)
-                        if (p.bias_tokens[f] == tok) s = __fadd_rn(s, p.bias_values[f]);
+            __syncwarp();
+            work_off(marks, mask, t0);
+            // ---- the span's tokens with a bias, once their raw logits are stored
+            if (r.b1 > r.b0 && (t0 + LG_CHUNK >= own || t0 + LG_CHUNK == c0 + r.span)) {
+                __syncthreads();
+                for (int e = r.b0 + tid; e < r.b1; e += LG_THREADS) {
+                    const int tok = p.bias_tokens[e], i = place_of(p, tok);
+                    if ((unsigned)(i - c0) >= (unsigned)r.span) continue;
+                    const uint32_t c = counters.get(i - c0);
+                    float s = p.bias_values[e];
+                    const float v = r.src[tok];  // in place: still the logit
+                    if (c & counters.again()) {  // the token's first entry adds up all of them, in order
+                        int f = r.b0;
+                        while (f < e && p.bias_tokens[f] != tok) f++;
+                        if (f < e) continue;
+                        for (f = e + 1; f < r.b1; f++)
+                            if (p.bias_tokens[f] == tok) s = __fadd_rn(s, p.bias_values[f]);
+                    }
+                    settle(tok, allowed_token(r, tok) ? constrained(p, r, v, c, s) : -INFINITY);
                 }
-                settle(tok, c, s);
             }
-            if (more) __syncthreads();  // the next stream reuses the list
         }
     }
-    return best;
+    return better(best, top);
 }
 
 // VEC: rows are 16-byte aligned (4 consecutive tokens per load); else one token per load, the warp's consecutive.
 // COUNT: the call has histories or biases.
 template <bool VEC, bool COUNT>
 __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParams p) {
-    extern __shared__ __align__(16) uint32_t counts[];  // p.count_bytes, then the list
+    extern __shared__ __align__(16) uint32_t counts[];  // p.count_bytes, then the bitmap, then the list
     __shared__ Best warp_best[LG_THREADS / 32];
     __shared__ __align__(8) Best candidate[LG_CLUSTER];  // in the first CTA: every CTA's
     __shared__ __align__(8) uint64_t pushed;
-    __shared__ int n_listed[2];
     const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x, row = blockIdx.y;
     const bool push = p.choice && C > 1;
     if (COUNT) {
-        for (int i = tid; i < p.count_bytes / 16; i += LG_THREADS) reinterpret_cast<uint4 *>(counts)[i] = uint4{0, 0, 0, 0};
-        if (tid < 2) n_listed[tid] = 0;
+        for (int i = tid; i < zero_units(p); i += LG_THREADS) reinterpret_cast<uint4 *>(counts)[i] = uint4{0, 0, 0, 0};
     }
     if (push) {  // the barrier for the candidates, set up before any CTA can arrive on it
         if (rank == 0 && tid == 0) {
@@ -331,12 +412,11 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
     grid_dependency_wait();
     grid_dependents_launch();
 
-    // the first logits are under way before anything waits for the lists' offsets
     Row r{};
     r.src = p.logits + (long long)row * p.logits_stride;
     r.dst = p.out ? p.out + (long long)row * p.out_stride : nullptr;
     float x[LG_LOADS][4];
-    load_chunk<VEC>(p, r.src, 0, x);
+    load_chunk<VEC>(p, r.src, 0, x);  // under way before anything waits for the lists' offsets
     const bool report = rank == 0 && tid == 0;
     if (p.mask) {
         const int m = p.mask_rows ? p.mask_rows[row] : row;
@@ -348,14 +428,16 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
         const int prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
         list_range(p.token_offsets, row, p.n_tokens, p.err, report, r.h0, r.h1);
         r.prompt_end = r.h0 + min(max(prompt, 0), r.h1 - r.h0);
+        if (p.repetition) r.repetition = p.repetition[row];
+        if (p.frequency) r.frequency = p.frequency[row];
+        if (p.presence) r.presence = p.presence[row];
     }
     if (COUNT && p.bias_tokens) list_range(p.bias_offsets, row, p.n_bias, p.err, report, r.b0, r.b1);
-    uint16_t *list = reinterpret_cast<uint16_t *>(reinterpret_cast<uint8_t *>(counts) + p.count_bytes);
-    Best best;
-    if (!COUNT || r.h1 - r.h0 <= LG_SHORT)
-        best = work_row<VEC, COUNT, true>(p, r, row, p.count_bytes / 2, counts, list, n_listed, x);
-    else
-        best = work_row<VEC, COUNT, false>(p, r, row, p.count_bytes / 4, counts, list, n_listed, x);
+    uint32_t *bitmap = counts + p.count_bytes / 4;
+    uint32_t *lists = bitmap + p.count_bytes / 64;  // a word per entry while the history is counted
+    r.counters = Counters{counts, r.h1 - r.prompt_end <= LG_SHORT};
+    r.span = r.counters.half ? p.count_bytes / 2 : p.count_bytes / 4;
+    Best best = work_row<VEC, COUNT>(p, r, bitmap, lists, x);
 
     // ---- the greedy choice
     if (!p.choice) return;
@@ -389,9 +471,11 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
     if (tid == 0) p.choice[row] = best.token;
 }
 
+size_t logits_smem(int count_bytes) { return count_bytes + count_bytes / 16 + (LG_WARPS * LG_LIST + LG_STAGE) * 4; }
+
 template <bool VEC, bool COUNT>
 int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
-    const size_t smem = COUNT ? p.count_bytes + LG_CHUNK * sizeof(uint16_t) : 0;
+    const size_t smem = COUNT ? logits_smem(p.count_bytes) : 0;
     {
         // the shared-memory and cluster-size opt-ins are per-device function attributes
         static std::mutex mu;
@@ -402,7 +486,7 @@ int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[dev]) {
             e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     LG_COUNT_BYTES_MAX + LG_CHUNK * (int)sizeof(uint16_t));
+                                     (int)logits_smem(LG_COUNT_BYTES_MAX));
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return fail_cuda(e, "tqk_process_logits: kernel attributes");

@@ -383,12 +383,13 @@ def decode(args: DecodeArgs, workspace=None, stream=None) -> None:
 
 def weights_args(weight, weight_out=None, *, item_stride=0, position=None, new_pos=None, new_pos0=0) -> WeightsArgs:
     """tqk_weights_args: running sums [..., n_kv, max_tokens] (fp32) and their positions (int32).  weight_out None
-    adds in place."""
+    adds in place.  The struct keeps its tensors alive."""
     w = WeightsArgs()
     w.weight = _typed(weight, "float32")
     w.weight_out = w.weight if weight_out is None else _typed(weight_out, "float32")
     w.item_stride = item_stride
     w.position, w.new_pos, w.new_pos0 = _typed(position, "int32"), _typed(new_pos, "int32"), new_pos0
+    w._keep = (weight, weight_out, position, new_pos)  # noqa: SLF001  (the struct holds bare addresses)
     return w
 
 
@@ -410,7 +411,7 @@ def decode_weights_workspace_size(args: DecodeArgs) -> int:
 def evict_args(k, v, n_kv, head_dim, max_tokens, budget, *, weight, weight_out=None, position=None, position_out=None,
                n_items=1, item_stride_blocks=0, stat_item_stride=0, lens=None, len0=0, len_step=0, max_len=0, n_first=0,
                n_recent=0, lens_out=None) -> EvictArgs:
-    """tqk_evict_args.  weight_out / position_out None: in place."""
+    """tqk_evict_args.  weight_out / position_out None: in place.  The struct keeps its tensors alive."""
     a = EvictArgs()
     a.k, a.v, a.item_stride = _ptr(k), _ptr(v), item_stride_blocks
     a.n_items, a.n_kv_heads, a.head_dim, a.max_tokens = n_items, n_kv, head_dim, max_tokens
@@ -423,6 +424,7 @@ def evict_args(k, v, n_kv, head_dim, max_tokens, budget, *, weight, weight_out=N
     a.position_out = a.position if position_out is None else _typed(position_out, "int32")
     a.stat_item_stride = stat_item_stride
     a.lens_out = _typed(lens_out, "int32")
+    a._keep = (k, v, weight, weight_out, position, position_out, lens, lens_out)  # noqa: SLF001
     return a
 
 
@@ -444,7 +446,8 @@ def logits_args(logits, *, out=None, choice=None, tokens=None, token_offsets=Non
                 repetition=None, frequency=None, presence=None, bias_tokens=None, bias_values=None, bias_offsets=None,
                 n_bias=None, mask=None, mask_rows=None) -> LogitsArgs:
     """tqk_logits_args from logits [n_rows, vocab] (rows may be strided), out likewise (None: only the choice),
-    packed histories and bias lists with their offsets [n_rows + 1], and mask words [n_mask_rows, words] (int32)."""
+    packed histories and bias lists with their offsets [n_rows + 1], and mask words [n_mask_rows, words] (int32).  The
+    struct keeps its tensors alive."""
     a = LogitsArgs()
     a.logits, a.logits_stride, a.n_rows, a.vocab_size = _row_ptr(logits, "float32")
     if out is not None:
@@ -463,6 +466,8 @@ def logits_args(logits, *, out=None, choice=None, tokens=None, token_offsets=Non
         if words < (a.vocab_size + 31) // 32:
             raise ValueError("mask rows need a bit per token")
     a.mask_rows = _typed(mask_rows, "int32")
+    a._keep = (logits, out, choice, tokens, token_offsets, prompt_lens, repetition, frequency, presence,  # noqa: SLF001
+               bias_tokens, bias_values, bias_offsets, mask, mask_rows)
     return a
 
 

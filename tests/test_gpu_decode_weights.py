@@ -304,6 +304,21 @@ def test_captured_and_replayed_on_two_streams(tqk, cuda):
             assert torch.equal(c.out, out) and torch.equal(c.dw.view(torch.int32), dw.view(torch.int32))
 
 
+def test_capture_needs_a_workspace(tqk, cuda):
+    import torch
+    c = Case(tqk, 65, 8, 2, 128, 100, [100])
+    tqk.decode_weights(c.args(), c.wargs())
+    torch.cuda.synchronize()
+    s, g, x = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+    with torch.cuda.graph(g, stream=s):
+        x.add_(1)
+        with pytest.raises(tqk.TQKError) as e:
+            tqk.decode_weights(c.args(), c.wargs())
+        assert e.value.status == tqk.EWORKSPACE
+    g.replay()
+    assert x.item() == 1
+
+
 def test_library_workspace_on_another_stream(tqk, cuda):
     import torch
     c = Case(tqk, 71, 32, 8, 128, 900, [900])

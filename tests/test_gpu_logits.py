@@ -190,3 +190,54 @@ def test_captured_with_changing_lists(tqk, cuda):
             for r in range(rows):
                 ref, best = logits_ref(x[r].cpu().numpy(), tokens=ids[r], repetition=1.5)
                 assert np.array_equal(out[r].cpu().numpy(), ref) and choice[r].item() == best
+
+
+@pytest.mark.parametrize("vocab", [9000, 70000, 131072, 300001])
+def test_every_token_in_the_history(tqk, cuda, vocab):
+    """More marked tokens than a warp lists at a time, and a hot token whose count passes 16 bits."""
+    import torch
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((2, vocab), dtype=np.float32)
+    hot = np.full(70000, 7, np.int32)
+    lists = [rng.permutation(vocab).astype(np.int32), np.concatenate([hot, np.arange(0, vocab, 3, dtype=np.int32)])]
+    off = np.concatenate([[0], np.cumsum([len(v) for v in lists])]).astype(np.int32)
+    prompts = np.array([vocab // 2, 11], np.int32)
+    allowed = rng.random((2, vocab)) < 0.7
+    bias = [[(5, 1.0), (vocab - 1, 2.0)], [(7, 40000.0), (8, -1.0), (7, 0.5)]]
+    dx = torch.from_numpy(x).cuda()
+    out, choice = torch.empty_like(dx), torch.empty(2, dtype=torch.int32, device="cuda")
+
+    def dev(a, t=None):
+        return torch.from_numpy(np.asarray(a, t)).cuda()
+
+    tqk.process_logits(tqk.logits_args(
+        dx, out=out, choice=choice, tokens=dev(np.concatenate(lists)), token_offsets=dev(off), prompt_lens=dev(prompts),
+        repetition=dev([1.25, 1.5], np.float32), frequency=dev([0.25, 0.5], np.float32), presence=dev([0.125, 0.75], np.float32),
+        bias_tokens=dev([t for b in bias for t, _ in b], np.int32), bias_values=dev([v for b in bias for _, v in b], np.float32),
+        bias_offsets=dev([0, 2, 5], np.int32), mask=dev(pack_bits(allowed))))
+    for r in range(2):
+        ref, best = logits_ref(x[r], tokens=lists[r], prompt=int(prompts[r]), repetition=[1.25, 1.5][r],
+                               frequency=[0.25, 0.5][r], presence=[0.125, 0.75][r], bias=bias[r], allowed=allowed[r])
+        assert np.array_equal(out[r].cpu().numpy().view(np.uint32), ref.view(np.uint32)) and choice[r].item() == best
+
+
+def test_histories_at_any_address(tqk, cuda):
+    """Token arrays that start 0 to 3 words into a 16-byte unit, with lists that start and end anywhere."""
+    import torch
+    rng = np.random.default_rng(4)
+    vocab, rows = 5003, 4
+    x = rng.standard_normal((rows, vocab), dtype=np.float32)
+    dx, buf = torch.from_numpy(x).cuda(), torch.zeros(12000, dtype=torch.int32, device="cuda")
+    for shift in range(4):
+        lens = rng.integers(0, 2500, rows)
+        off = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+        ids = rng.integers(0, vocab, off[-1]).astype(np.int32)
+        tokens = buf[shift:shift + max(1, len(ids))]
+        tokens[:len(ids)] = torch.from_numpy(ids).cuda()
+        rep = rng.random(rows, dtype=np.float32) + 1
+        out, choice = torch.empty_like(dx), torch.empty(rows, dtype=torch.int32, device="cuda")
+        tqk.process_logits(tqk.logits_args(dx, out=out, choice=choice, tokens=tokens, n_tokens=len(ids),
+                                           token_offsets=torch.from_numpy(off).cuda(), repetition=torch.from_numpy(rep).cuda()))
+        for r in range(rows):
+            ref, best = logits_ref(x[r], tokens=ids[off[r]:off[r + 1]], repetition=rep[r])
+            assert np.array_equal(out[r].cpu().numpy(), ref) and choice[r].item() == best
