@@ -254,9 +254,18 @@ __device__ __forceinline__ void pack_step(PackState<NB> &st, const uint8_t *k_a,
     {                                                                                           \
         float *a = st.acc[b][JJ];                                                               \
         const uint32_t x0 = s8pair_to_f16x2<JJ>(wa0, wa1), y0 = s8pair_to_f16x2<JJ>(wb0, wb1);  \
-        mma_f16_k16_hl(a[0], a[1], h0a, l0a, h0b, l0b, x0, y0);                                 \
         const uint32_t x1 = s8pair_to_f16x2<JJ>(wa8, wa9), y1 = s8pair_to_f16x2<JJ>(wb8, wb9);  \
-        mma_f16_k16_hl(a[0], a[1], h1a, l1a, h1b, l1b, x1, y1);                                 \
+        if constexpr (WT != WT_NONE) {                                                          \
+            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};                                     \
+            float s[4], d[4];                                                                   \
+            mma_f16_k16_step(s, zero, h0a, l0a, h0b, l0b, x0, y0);                              \
+            mma_f16_k16_step(d, s, h1a, l1a, h1b, l1b, x1, y1);                                 \
+            a[0] += d[0] + d[2];                                                                \
+            a[1] += d[1] + d[3];                                                                \
+        } else {                                                                                \
+            mma_f16_k16_hl(a[0], a[1], h0a, l0a, h0b, l0b, x0, y0);                             \
+            mma_f16_k16_hl(a[0], a[1], h1a, l1a, h1b, l1b, x1, y1);                             \
+        }                                                                                       \
     }
         TQK_PK_NTILE(0)
         TQK_PK_NTILE(1)

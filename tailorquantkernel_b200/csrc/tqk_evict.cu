@@ -22,7 +22,7 @@
 //      into a list that overwrites the keys;
 //   4. the moves are dealt out evenly over the cluster's CTAs, which look up the
 //      j-th hole and the j-th mover in the CTAs' lists and copy the rows; every warp
-//      works on moves of its own, 8 of them in flight.
+//      works on moves of its own, 4 of them in flight.
 // Only integer counts are summed, so results do not depend on timing.
 #include "tqk_internal.h"
 
@@ -37,13 +37,10 @@ constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;                   // histogram bins: digits of 11, 11 and 10 bits
 constexpr int EV_RUN_MAX = 63;                  // slots per thread: a bit each of a 64-bit mask, an odd number
-constexpr int EV_CLUSTER_MAX = 16;              // non-portable above 8
-constexpr int EV_UNITS = 8;                     // 16-byte units in flight per thread
+constexpr int EV_CLUSTER_MAX = 8;               // the portable cluster size
+constexpr int EV_UNITS = 4;                     // units in flight per thread; a ragged batch, 2, 4, 8: 127, 105, 118 us
 constexpr int EV_LOADS = 8;                     // sums and positions in flight per thread
 constexpr int EV_ALONE = 100 << 10;             // dynamic shared memory that leaves no room for a second CTA
-#ifndef EVPER
-#define EVPER 8192
-#endif
 constexpr int EV_STAGE = 8192;                  // slots per CTA whose positions are staged in shared memory
 static_assert(EV_CLUSTER_MAX * EV_THREADS * EV_RUN_MAX == TQK_EVICT_MAX_LEN, "documented limit");
 
@@ -107,7 +104,7 @@ __device__ __forceinline__ int block_prefix(int v, int *warp_tot, int *total) {
 // One warp moves rows of both planes from slots src to slots dst, lane l's move in its src and dst, the first n lanes'.
 // A row is 9 16-byte units (9 words for head_dim 32), or twice as many; K's and V's units lie next to each other in the
 // lanes where both fit, so a lane's place in the row never changes and a move costs one load and one store.  Denser
-// layouts (every lane at work, twice the bytes in flight) were slower: 128 us against 119 us for a ragged batch.
+// layouts (every lane at work, twice the bytes in flight) were slower: 128 us against 118 us for a ragged batch.
 template <int NB>
 __device__ __forceinline__ void move_rows(uint8_t *kh, uint8_t *vh, int src, int dst, int n) {
     constexpr int ROW = NB * BLOCK_BYTES;
@@ -173,8 +170,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
     const int run = ((len + C * EV_THREADS - 1) / (C * EV_THREADS)) | 1;
     const int s0 = min(len, rank * run * EV_THREADS), s1 = min(len, s0 + run * EV_THREADS), n_own = s1 - s0;
     auto cluster_barrier = [&]() {
+        __syncthreads();  // the cluster barrier's instructions meet converged warps
         if (C > 1) cluster_sync_all();
-        else __syncthreads();
     };
 
     if (len <= budget) {  // nothing to evict (the same for every CTA of the cluster)
@@ -278,7 +275,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
                 if (x.z) atomicAdd(&hist[bin + 2], x.z);
                 if (x.w) atomicAdd(&hist[bin + 3], x.w);
             }
-            cluster_sync_all();
+            cluster_barrier();
         }
         // thread t takes the t-th four bins from the top
         uint4 cnt{0, 0, 0, 0};
@@ -310,7 +307,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
         tie_rank = block_prefix(ties, sh.warp_tot[3], &all);
         if (C > 1) {
             if (tid == 0) sh.ties = all;
-            cluster_sync_all();
+            cluster_barrier();
             const int r = tid & 31;
             const int x = r < rank ? (int)ld_cluster_u32(cluster_map(&sh.ties, (uint32_t)r)) : 0;
             tie_rank += __reduce_add_sync(0xffffffffu, x);
@@ -360,8 +357,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
     }
     __syncthreads();
 
-    // ---- 4. this CTA's share of the moves (holes and movers are equally many)
-    const long long n_moves = sh.pre_m[C];
+    // ---- 4. this CTA's share of the moves (holes and movers are equally many; nothing moves if they should not be)
+    const long long n_moves = sh.pre_m[C] == sh.pre_h[C] ? sh.pre_m[C] : 0;
     const int m0 = (int)(n_moves * rank / C), m1 = (int)(n_moves * (rank + 1) / C);
     const long long head_off = (long long)item * p.item_stride + (long long)kvh * p.max_tokens * (NB * BLOCK_BYTES);
     // up to 32 moves at a time per warp, a lane looking each of them up
@@ -383,7 +380,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
         }
         move_rows<NB>(p.k + head_off, p.v + head_off, src, dst, n);
     }
-    if (C > 1) cluster_sync_all();  // no CTA leaves while another reads its list
+    if (C > 1) cluster_barrier();  // no CTA leaves while another reads its list
 }
 
 // lens_out[i] = min(len_i, budget) in place: after the eviction has read every length.
@@ -397,9 +394,9 @@ __global__ void evict_lens_kernel(const int *lens, int len0, int len_step, int l
 template <int NB>
 int launch_evict(const EvictParams &p, int cluster, dim3 grid, cudaStream_t stream) {
     size_t smem = (size_t)EV_THREADS * p.run * (p.staged ? 2 : 1) * sizeof(uint32_t);
-    // few CTAs: one per SM (two would share an SM while others idle); the largest clusters do not fit a GPC that way
-    if (cluster <= 8 && (long long)grid.x * grid.y * grid.z <= device_info()->sm_count && smem < EV_ALONE) smem = EV_ALONE;
-    // the shared-memory and cluster-size opt-ins are per-device function attributes
+    // few CTAs: one per SM (two would share an SM while others idle)
+    if ((long long)grid.x * grid.y * grid.z <= device_info()->sm_count && smem < EV_ALONE) smem = EV_ALONE;
+    // the dynamic shared-memory opt-in is a per-device function attribute
     static std::mutex mu;
     static bool ready[64];
     int dev = 0;
@@ -410,8 +407,6 @@ int launch_evict(const EvictParams &p, int cluster, dim3 grid, cudaStream_t stre
         if (!ready[dev]) {
             e = cudaFuncSetAttribute(evict_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      EV_THREADS * EV_RUN_MAX * (int)sizeof(uint32_t));
-            if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(evict_kernel<NB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return fail_cuda(e, "tqk_evict_q8: kernel attributes");
             ready[dev] = true;
         }
@@ -487,10 +482,10 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
         p.position_out = a->position_out;
         p.stat_stride = a->stat_item_stride;
         p.err = device_info()->err_word;
-        // CTAs per (item, head): one up to 8192 slots (clusters cost more than they bring there), then as many as hold
+        // CTAs per (item, head): one up to 8192 slots (32 layers at 4097: 11 us, with two 27 us), then as many as hold
         // 8192 each, as far as a cluster goes
         int cluster = 1;
-        while (cluster < EV_CLUSTER_MAX && cluster * EVPER < max_len) cluster *= 2;
+        while (cluster < EV_CLUSTER_MAX && cluster * EV_STAGE < max_len) cluster *= 2;
         p.run = ((max_len + cluster * EV_THREADS - 1) / (cluster * EV_THREADS)) | 1;
         p.staged = max_len <= cluster * EV_STAGE;
         p.lens_out = a->lens_out != a->lens ? a->lens_out : nullptr;

@@ -86,7 +86,7 @@ EVICT = dict(k=FAKE, v=FAKE, weight=FAKE, weight_out=FAKE, position=FAKE, positi
     (dict(len0=65), "EPOS"), (dict(len0=-1), "EPOS"), (dict(len_step=5), "EPOS"), (dict(lens=FAKE, max_len=65), "EINVAL"),
     (dict(lens=FAKE, max_len=-1), "EINVAL"), (dict(k=FAKE + 4), "EALIGN"), (dict(item_stride=513), "EALIGN"),
     (dict(head_dim=64, k=FAKE + 2), "EALIGN"), (dict(weight=FAKE + 2), "EALIGN"), (dict(position_out=FAKE + 1), "EALIGN"),
-    (dict(n_items=1, max_tokens=600000, len0=520000), "EUNSUPPORTED"),
+    (dict(n_items=1, max_tokens=600000, len0=258049), "EUNSUPPORTED"),
     (dict(n_items=70000), "EINVAL"),
 ])
 def test_evict_refusals(tqk, change, status):

@@ -41,8 +41,9 @@ CASES = [  # nkv, hd, mt, lens, device lens, budget, first, recent, weights, pos
     (2, 128, 9000, [9000], False, 100, 4, 32, "normal", "rising"),       # two CTAs per head
     (1, 128, 40000, [40000, 20000], True, 19999, 0, 1000, "ties", "mixed"),
     (2, 32, 70001, [70001], False, 70000, 3, 500, "equal", "mixed"),
-    (1, 32, 300000, [300000], False, 1234, 4, 100, "normal", "rising"),  # the largest clusters
-    (1, 32, 300000, [300000], False, 299000, 0, 0, "ties", None),
+    (1, 32, 258048, [258048], False, 1234, 4, 100, "normal", "rising"),  # the longest
+    (1, 32, 250001, [250001], False, 249000, 0, 0, "ties", None),
+    (2, 128, 140001, [140001], False, 50000, 4, 1000, "normal", "mixed"),
     (2, 64, 513, [513], False, 200, 0, 0, "odd", None),
     (2, 64, 9001, [9001], False, 4000, 10, 10, "odd", "mixed"),
     (2, 128, 1000, [1000], False, 500, 0, 0, "equal", "mixed"),
