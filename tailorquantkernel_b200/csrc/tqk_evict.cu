@@ -33,14 +33,16 @@
 namespace tqk {
 namespace {
 
-constexpr int EV_THREADS = 512;
-constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_THREADS = 512;                 // per CTA; EV_WIDE where a long length has an SM for every CTA
+constexpr int EV_WIDE = 1024;
 constexpr int EV_BINS = 2048;                   // histogram bins: digits of 11, 11 and 10 bits
 constexpr int EV_RUN_MAX = 63;                  // slots per thread: a bit each of a 64-bit mask, an odd number
 constexpr int EV_CLUSTER_MAX = 8;               // the portable cluster size
 constexpr int EV_UNITS = 4;                     // units in flight per thread; a ragged batch, 2, 4, 8: 127, 105, 118 us
 constexpr int EV_LOADS = 8;                     // sums and positions in flight per thread
 constexpr int EV_ALONE = 100 << 10;             // dynamic shared memory that leaves no room for a second CTA
+constexpr int EV_KEY_BYTES_MAX = 140 << 10;     // dynamic shared memory at the longest length
+constexpr int EV_NARROW = 1024;                 // slots per CTA where every CTA has an SM
 constexpr int EV_STAGE = 8192;                  // slots per CTA whose positions are staged in shared memory
 static_assert(EV_CLUSTER_MAX * EV_THREADS * EV_RUN_MAX == TQK_EVICT_MAX_LEN, "documented limit");
 
@@ -62,9 +64,10 @@ struct EvictParams {
     int *err;
 };
 
+template <int T>
 struct EvictShared {
     __align__(16) unsigned hist[3][EV_BINS];
-    int warp_tot[6][EV_WARPS];   // of each block_prefix: a buffer of its own saves a barrier
+    int warp_tot[5][T / 32];   // of each block_prefix: a buffer of its own saves a barrier
     int max_pos;                 // this CTA's largest position
     int counts[2];               // this CTA's holes and movers
     int ties;                    // this CTA's keys equal to the threshold
@@ -83,6 +86,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 constexpr uint32_t KEY_PROTECTED = 0xFFFFFFFFu;  // above +inf's 0xFF800000
 
 // Exclusive prefix sum of v over the CTA's threads; *total receives the sum.  warp_tot: a buffer that no other call uses.
+template <int T>
 __device__ __forceinline__ int block_prefix(int v, int *warp_tot, int *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int incl = v;
@@ -94,7 +98,7 @@ __device__ __forceinline__ int block_prefix(int v, int *warp_tot, int *total) {
     if (lane == 31) warp_tot[warp] = incl;
     __syncthreads();
     // the warps' totals, one per lane
-    int before = lane < EV_WARPS ? warp_tot[lane] : 0, all = before;
+    int before = lane < T / 32 ? warp_tot[lane] : 0, all = before;
     if (lane >= warp) before = 0;
     before = __reduce_add_sync(0xffffffffu, before);
     *total = __reduce_add_sync(0xffffffffu, all);
@@ -138,12 +142,12 @@ __device__ __forceinline__ void move_rows(uint8_t *kh, uint8_t *vh, int src, int
     }
 }
 
-template <int NB>
-__global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams p) {
-    extern __shared__ __align__(16) uint32_t keys[];  // [EV_THREADS * run], then the slots of holes and movers
-    __shared__ EvictShared sh;
+template <int NB, int T>
+__global__ void __launch_bounds__(T, 1024 / T) evict_kernel(const EvictParams p) {
+    extern __shared__ __align__(16) uint32_t keys[];  // [T * run], then the slots of holes and movers
+    __shared__ EvictShared<T> sh;
     const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x;
-    for (int i = tid; i < 3 * EV_BINS / 4; i += EV_THREADS) reinterpret_cast<uint4 *>(sh.hist)[i] = uint4{0, 0, 0, 0};
+    for (int i = tid; i < 3 * EV_BINS / 4; i += T) reinterpret_cast<uint4 *>(sh.hist)[i] = uint4{0, 0, 0, 0};
     if (tid == 0) {
         sh.max_pos = INT_MIN;
         sh.n_close = 0;
@@ -167,15 +171,15 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
     const bool copy_w = w_out != w_in, copy_pos = pos_out != pos_in;
     // this CTA's slots [s0, s1), `run` consecutive ones per thread; an odd run keeps the threads' shared-memory
     // words in different banks
-    const int run = ((len + C * EV_THREADS - 1) / (C * EV_THREADS)) | 1;
-    const int s0 = min(len, rank * run * EV_THREADS), s1 = min(len, s0 + run * EV_THREADS), n_own = s1 - s0;
+    const int run = ((len + C * T - 1) / (C * T)) | 1;
+    const int s0 = min(len, rank * run * T), s1 = min(len, s0 + run * T), n_own = s1 - s0;
     auto cluster_barrier = [&]() {
         __syncthreads();  // the cluster barrier's instructions meet converged warps
         if (C > 1) cluster_sync_all();
     };
 
     if (len <= budget) {  // nothing to evict (the same for every CTA of the cluster)
-        for (int i = s0 + tid; i < s1; i += EV_THREADS) {
+        for (int i = s0 + tid; i < s1; i += T) {
             if (copy_w) w_out[i] = w_in[i];
             if (copy_pos) pos_out[i] = pos_in[i];
         }
@@ -185,20 +189,20 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
     // ---- 1. keys.  Protection needs the newest position first: the positions wait in shared memory behind the keys,
     //         or, from EV_STAGE slots per CTA on, are read again
     const bool recent = p.n_recent > 0, staged = p.staged;
-    int *pos_s = reinterpret_cast<int *>(keys) + EV_THREADS * p.run;
+    int *pos_s = reinterpret_cast<int *>(keys) + T * p.run;
     int newest = INT_MIN;
-    for (int i0 = tid; i0 < n_own; i0 += EV_LOADS * EV_THREADS) {
+    for (int i0 = tid; i0 < n_own; i0 += EV_LOADS * T) {
         float w[EV_LOADS];
         int pos[EV_LOADS];
 #pragma unroll
         for (int q = 0; q < EV_LOADS; q++) {
-            const int s = s0 + i0 + q * EV_THREADS;
+            const int s = s0 + i0 + q * T;
             w[q] = s < s1 ? w_in[s] : 0.0f;
             pos[q] = pos_in && s < s1 ? pos_in[s] : INT_MIN;
         }
 #pragma unroll
         for (int q = 0; q < EV_LOADS; q++) {
-            const int i = i0 + q * EV_THREADS, s = s0 + i;
+            const int i = i0 + q * T, s = s0 + i;
             if (i >= n_own) break;
             newest = max(newest, pos[q]);
             keys[i] = pos_in && pos[q] < p.n_first ? KEY_PROTECTED : weight_key(w[q]);
@@ -218,18 +222,18 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
     }
     // the first digit's histogram, from the final keys (each thread its own slots')
     const long long recent_from = (long long)newest - p.n_recent;  // positions above are protected
-    for (int i0 = tid; i0 < n_own; i0 += EV_LOADS * EV_THREADS) {
+    for (int i0 = tid; i0 < n_own; i0 += EV_LOADS * T) {
         int pos[EV_LOADS];
         if (recent) {
 #pragma unroll
             for (int q = 0; q < EV_LOADS; q++) {
-                const int i = i0 + q * EV_THREADS;
+                const int i = i0 + q * T;
                 pos[q] = i >= n_own ? INT_MIN : staged ? pos_s[i] : pos_in[s0 + i];
             }
         }
 #pragma unroll
         for (int q = 0; q < EV_LOADS; q++) {
-            const int i = i0 + q * EV_THREADS;
+            const int i = i0 + q * T;
             if (i >= n_own) break;
             uint32_t key = keys[i];
             if (recent && pos[q] > recent_from) keys[i] = key = KEY_PROTECTED;
@@ -242,13 +246,13 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
     uint32_t prefix = 0;
     int need = budget, equal = 0;
     uint32_t *close = reinterpret_cast<uint32_t *>(pos_s);  // the keys that share two digits, as far as they fit
-    const int close_cap = staged ? EV_THREADS * p.run : 0;
+    const int close_cap = staged ? T * p.run : 0;
 #pragma unroll
     for (int digit = 0; digit < 3; digit++) {
         const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bins = digit == 2 ? 1024 : 2048;
         unsigned *hist = sh.hist[digit];
         if (digit == 1) {
-            for (int i = tid; i < n_own; i += EV_THREADS) {
+            for (int i = tid; i < n_own; i += T) {
                 const uint32_t key = keys[i];
                 if (key >> 21 != prefix >> 21) continue;
                 atomicAdd(&hist[(key >> 10) & 2047], 1u);
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
             const bool listed = sh.n_close <= close_cap;
             const uint32_t *from = listed ? close : keys;
             const int n = listed ? sh.n_close : n_own;
-            for (int i = tid; i < n; i += EV_THREADS)
+            for (int i = tid; i < n; i += T)
                 if (from[i] >> 10 == prefix >> 10) atomicAdd(&hist[from[i] & 1023], 1u);
         }
         cluster_barrier();
@@ -281,7 +285,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
         uint4 cnt{0, 0, 0, 0};
         const int bin0 = bins - 4 - 4 * tid;
         if (bin0 >= 0) cnt = ld_cluster_u32x4(cluster_map(hist + bin0, (uint32_t)(bin0 / share)));
-        int all, above = block_prefix((int)(cnt.x + cnt.y + cnt.z + cnt.w), sh.warp_tot[digit], &all);
+        int all, above = block_prefix<T>((int)(cnt.x + cnt.y + cnt.z + cnt.w), sh.warp_tot[digit], &all);
         const int c4[4] = {(int)cnt.w, (int)cnt.z, (int)cnt.y, (int)cnt.x};
 #pragma unroll
         for (int q = 0; q < 4; q++) {
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
     if (equal > need) {
         int ties = 0, all;
         for (int i = r0; i < r1; i++) ties += keys[i] == prefix;
-        tie_rank = block_prefix(ties, sh.warp_tot[3], &all);
+        tie_rank = block_prefix<T>(ties, sh.warp_tot[3], &all);
         if (C > 1) {
             if (tid == 0) sh.ties = all;
             cluster_barrier();
@@ -322,15 +326,15 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
         if (s0 + i < budget) holes |= keep ? 0ull : bit;
         else movers |= keep ? bit : 0ull;
     }
-    // at most 32256 slots per CTA: both counts fit in half a word
+    // at most 33792 slots per CTA: both counts fit in half an unsigned word
     int both;
-    const int ranks = block_prefix((__popcll(holes) << 16) | __popcll(movers), sh.warp_tot[4], &both);
+    const uint32_t ranks = (uint32_t)block_prefix<T>((int)((uint32_t)__popcll(holes) << 16) | __popcll(movers), sh.warp_tot[4], &both);
     int *list = reinterpret_cast<int *>(keys);  // every key is read: holes from the front, movers from the back
-    const int last = EV_THREADS * run - 1;
-    for (int j = ranks >> 16; holes; holes &= holes - 1) list[j++] = s0 + r0 + __ffsll(holes) - 1;
-    for (int j = ranks & 0xFFFF; movers; movers &= movers - 1) list[last - j++] = s0 + r0 + __ffsll(movers) - 1;
+    const int last = T * run - 1;
+    for (int j = (int)(ranks >> 16); holes; holes &= holes - 1) list[j++] = s0 + r0 + __ffsll(holes) - 1;
+    for (int j = (int)(ranks & 0xFFFFu); movers; movers &= movers - 1) list[last - j++] = s0 + r0 + __ffsll(movers) - 1;
     if (tid == 0) {
-        sh.counts[0] = both >> 16;
+        sh.counts[0] = (int)((uint32_t)both >> 16);
         sh.counts[1] = both & 0xFFFF;
     }
     cluster_barrier();
@@ -368,8 +372,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const EvictParams 
         return (int)ld_cluster_u32(cluster_map(mover ? &list[last - (j - pre[r])] : &list[j - pre[r]], (uint32_t)r));
     };
     // few moves are spread over the warps
-    const int lane = tid & 31, step = max(1, min(32, (m1 - m0 + EV_WARPS - 1) / EV_WARPS));
-    for (int b = m0 + (tid >> 5) * step; b < m1; b += EV_WARPS * step) {
+    const int lane = tid & 31, step = max(1, min(32, (m1 - m0 + (T / 32) - 1) / (T / 32)));
+    for (int b = m0 + (tid >> 5) * step; b < m1; b += (T / 32) * step) {
         const int n = min(step, m1 - b);
         int src = 0, dst = 0;
         if (lane < n) {
@@ -391,9 +395,9 @@ __global__ void evict_lens_kernel(const int *lens, int len0, int len_step, int l
     if (i < n) out[i] = min(min(max(lens ? lens[i] : len0 + i * len_step, 0), len_cap), budget);
 }
 
-template <int NB>
+template <int NB, int T>
 int launch_evict(const EvictParams &p, int cluster, dim3 grid, cudaStream_t stream) {
-    size_t smem = (size_t)EV_THREADS * p.run * (p.staged ? 2 : 1) * sizeof(uint32_t);
+    size_t smem = (size_t)T * p.run * (p.staged ? 2 : 1) * sizeof(uint32_t);
     // few CTAs: one per SM (two would share an SM while others idle)
     if ((long long)grid.x * grid.y * grid.z <= device_info()->sm_count && smem < EV_ALONE) smem = EV_ALONE;
     // the dynamic shared-memory opt-in is a per-device function attribute
@@ -405,14 +409,24 @@ int launch_evict(const EvictParams &p, int cluster, dim3 grid, cudaStream_t stre
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[dev]) {
-            e = cudaFuncSetAttribute(evict_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     EV_THREADS * EV_RUN_MAX * (int)sizeof(uint32_t));
+            e = cudaFuncSetAttribute(evict_kernel<NB, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     EV_KEY_BYTES_MAX);
             if (e != cudaSuccess) return fail_cuda(e, "tqk_evict_q8: kernel attributes");
             ready[dev] = true;
         }
     }
-    if (cluster == 1) return launch_pdl(evict_kernel<NB>, grid, dim3(EV_THREADS), smem, stream, p);
-    return launch_pdl_cluster(evict_kernel<NB>, grid, dim3(EV_THREADS), smem, stream, (unsigned)cluster, p);
+    if (cluster == 1) return launch_pdl(evict_kernel<NB, T>, grid, dim3(T), smem, stream, p);
+    return launch_pdl_cluster(evict_kernel<NB, T>, grid, dim3(T), smem, stream, (unsigned)cluster, p);
+}
+
+template <int T>
+int dispatch_evict(int nb, const EvictParams &p, int cluster, dim3 grid, cudaStream_t stream) {
+    switch (nb) {
+        case 1: return launch_evict<1, T>(p, cluster, grid, stream);
+        case 2: return launch_evict<2, T>(p, cluster, grid, stream);
+        case 4: return launch_evict<4, T>(p, cluster, grid, stream);
+        default: return launch_evict<8, T>(p, cluster, grid, stream);
+    }
 }
 
 }  // namespace
@@ -482,20 +496,23 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
         p.position_out = a->position_out;
         p.stat_stride = a->stat_item_stride;
         p.err = device_info()->err_word;
-        // CTAs per (item, head): one up to 8192 slots (32 layers at 4097: 11 us, with two 27 us), then as many as hold
-        // 8192 each, as far as a cluster goes
+        // CTAs per (item, head), as far as a cluster goes: as many as hold 8192 slots each (32 layers of 8 heads at 4097
+        // rows: 11 us with one, 27 us with two), and down to 1024 each while every CTA has an SM (8 heads, half of
+        // 8192 rows evicted: 31 us with one CTA per head, 17 us with eight).  Then also 1024 threads instead of 512,
+        // which bring the work per thread down and more moves in flight (8 heads, a quarter of 131072 rows kept: 87 and
+        // 69 us); up to 4096 slots they do not pay
         int cluster = 1;
         while (cluster < EV_CLUSTER_MAX && cluster * EV_STAGE < max_len) cluster *= 2;
-        p.run = ((max_len + cluster * EV_THREADS - 1) / (cluster * EV_THREADS)) | 1;
+        const long long units = (long long)a->n_items * a->n_kv_heads;
+        while (cluster < EV_CLUSTER_MAX && cluster * EV_NARROW < max_len && 2 * cluster * units <= device_info()->sm_count)
+            cluster *= 2;
+        const dim3 grid((unsigned)cluster, (unsigned)a->n_kv_heads, (unsigned)a->n_items);
+        const bool wide = max_len > EV_STAGE / 2 && (long long)grid.x * grid.y * grid.z <= device_info()->sm_count;
+        const int threads = wide ? EV_WIDE : EV_THREADS;
+        p.run = ((max_len + cluster * threads - 1) / (cluster * threads)) | 1;
         p.staged = max_len <= cluster * EV_STAGE;
         p.lens_out = a->lens_out != a->lens ? a->lens_out : nullptr;
-        const dim3 grid((unsigned)cluster, (unsigned)a->n_kv_heads, (unsigned)a->n_items);
-        switch (nb) {
-            case 1: rc = launch_evict<1>(p, cluster, grid, st); break;
-            case 2: rc = launch_evict<2>(p, cluster, grid, st); break;
-            case 4: rc = launch_evict<4>(p, cluster, grid, st); break;
-            default: rc = launch_evict<8>(p, cluster, grid, st); break;
-        }
+        rc = wide ? dispatch_evict<EV_WIDE>(nb, p, cluster, grid, st) : dispatch_evict<EV_THREADS>(nb, p, cluster, grid, st);
         if (rc) return rc;
     }
     if (!a->lens_out || (max_len > 0 && a->lens_out != a->lens)) return TQK_OK;

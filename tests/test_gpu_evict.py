@@ -44,6 +44,9 @@ CASES = [  # nkv, hd, mt, lens, device lens, budget, first, recent, weights, pos
     (1, 32, 258048, [258048], False, 1234, 4, 100, "normal", "rising"),  # the longest
     (1, 32, 250001, [250001], False, 249000, 0, 0, "ties", None),
     (2, 128, 140001, [140001], False, 50000, 4, 1000, "normal", "mixed"),
+    (1, 64, 258048, [258048], False, 129000, 0, 0, "normal", None),      # as many holes as a CTA can have
+    (1, 32, 258048, [258048], False, 60000, 0, 60000, "normal", "rising"),
+    (16, 32, 16500, [16500, 16499], False, 9000, 4, 100, "normal", "mixed"),  # more CTAs than SMs hold alone
     (2, 64, 513, [513], False, 200, 0, 0, "odd", None),
     (2, 64, 9001, [9001], False, 4000, 10, 10, "odd", "mixed"),
     (2, 128, 1000, [1000], False, 500, 0, 0, "equal", "mixed"),
