@@ -257,7 +257,7 @@ TQK_API int tqk_decode_q8_weights(const tqk_decode_args *a, const tqk_weights_ar
  *   - position may be NULL when n_first and n_recent are 0.
  *   - max_len at most TQK_EVICT_MAX_LEN.  Device lengths are clamped to max_len
  *     and reported as TQK_EDEVLEN.
- *   - No workspace; one launch, and one more with lens_out. */
+ *   - No workspace; one launch, and one more where lens_out is lens. */
 #define TQK_EVICT_MAX_LEN 258048
 typedef struct {
     tqk_block_q8 *k, *v;         /* planes of item 0 (device), [n_kv][max_tokens][head_dim/32] */

@@ -361,7 +361,8 @@ __global__ void __launch_bounds__(T, 1024 / T) evict_kernel(const EvictParams p)
     }
     __syncthreads();
 
-    // ---- 4. this CTA's share of the moves (holes and movers are equally many; nothing moves if they should not be)
+    // ---- 4. this CTA's share of the moves (holes and movers are equally many; if they should not be, nothing moves)
+    if (tid == 0 && sh.pre_m[C] != sh.pre_h[C]) record_error(p.err, DEVERR_BADLEN);
     const long long n_moves = sh.pre_m[C] == sh.pre_h[C] ? sh.pre_m[C] : 0;
     const int m0 = (int)(n_moves * rank / C), m1 = (int)(n_moves * (rank + 1) / C);
     const long long head_off = (long long)item * p.item_stride + (long long)kvh * p.max_tokens * (NB * BLOCK_BYTES);

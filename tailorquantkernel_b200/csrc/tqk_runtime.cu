@@ -37,6 +37,7 @@ void *grow_zeroed(Workspace &w, cudaStream_t stream, size_t bytes) {
     }
     size_t grow = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
     if (cudaMalloc(&w.ptr, grow) != cudaSuccess) {
+        (void)cudaGetLastError();  // reported by the caller; the next launch check must not find it
         w.ptr = nullptr;
         return nullptr;
     }

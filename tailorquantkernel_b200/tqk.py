@@ -97,12 +97,14 @@ tqk_decode_q8_static = _sig("tqk_decode_q8_static", [ctypes.POINTER(DecodeArgs),
 
 class WeightsArgs(ctypes.Structure):
     """Mirror of tqk_weights_args (include/tqk.h)."""
+    _device = None  # of the tensors it was made from, if any
     _fields_ = [("weight", _vp), ("weight_out", _vp), ("item_stride", _i64), ("position", _vp), ("new_pos", _vp),
                 ("new_pos0", _i)]
 
 
 class EvictArgs(ctypes.Structure):
     """Mirror of tqk_evict_args (include/tqk.h)."""
+    _device = None
     _fields_ = [
         ("k", _vp), ("v", _vp),
         ("item_stride", _i64),
@@ -121,6 +123,7 @@ class EvictArgs(ctypes.Structure):
 
 class LogitsArgs(ctypes.Structure):
     """Mirror of tqk_logits_args (include/tqk.h)."""
+    _device = None
     _fields_ = [
         ("logits", _vp), ("logits_stride", _i64),
         ("out", _vp), ("out_stride", _i64),
@@ -282,6 +285,23 @@ def _typed(t, dtype: str) -> Optional[int]:
     return _ptr(t)
 
 
+def _device_of(*tensors) -> Optional[int]:
+    """The CUDA device of the tensors among the arguments (None without any); they must share one."""
+    found = {t.device.index for t in tensors if t is not None and not isinstance(t, int)}
+    if len(found) > 1:
+        raise ValueError(f"tensors of one call on several devices: {sorted(found)}")
+    return found.pop() if found else None
+
+
+def _on_device(device: Optional[int]) -> None:
+    """The library launches on the current device: a call's tensors must live there."""
+    if device is not None:
+        import torch
+        if torch.cuda.current_device() != device:
+            raise ValueError(f"the call's tensors are on cuda:{device}, the current device is "
+                             f"cuda:{torch.cuda.current_device()}")
+
+
 def _stream(stream) -> int:
     import torch
     if stream is None:
@@ -390,11 +410,13 @@ def weights_args(weight, weight_out=None, *, item_stride=0, position=None, new_p
     w.item_stride = item_stride
     w.position, w.new_pos, w.new_pos0 = _typed(position, "int32"), _typed(new_pos, "int32"), new_pos0
     w._keep = (weight, weight_out, position, new_pos)  # noqa: SLF001  (the struct holds bare addresses)
+    w._device = _device_of(*w._keep)  # noqa: SLF001
     return w
 
 
 def decode_weights(args: DecodeArgs, weights: WeightsArgs, workspace=None, stream=None) -> None:
     """tqk_decode_q8_weights: the decode, and each cached row's attention weight added to its running sum."""
+    _on_device(weights._device)  # noqa: SLF001
     ws = _ptr(workspace) if workspace is not None else None
     nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     check(tqk_decode_q8_weights(ctypes.byref(args), ctypes.byref(weights), ws, nbytes, _stream(stream)),
@@ -425,11 +447,13 @@ def evict_args(k, v, n_kv, head_dim, max_tokens, budget, *, weight, weight_out=N
     a.stat_item_stride = stat_item_stride
     a.lens_out = _typed(lens_out, "int32")
     a._keep = (k, v, weight, weight_out, position, position_out, lens, lens_out)  # noqa: SLF001
+    a._device = _device_of(*a._keep)  # noqa: SLF001
     return a
 
 
 def evict(args: EvictArgs, stream=None) -> None:
     """tqk_evict_q8: every (item, kv head) goes down to its budget of rows."""
+    _on_device(args._device)  # noqa: SLF001
     check(tqk_evict_q8(ctypes.byref(args), _stream(stream)), "tqk_evict_q8")
 
 
@@ -468,11 +492,13 @@ def logits_args(logits, *, out=None, choice=None, tokens=None, token_offsets=Non
     a.mask_rows = _typed(mask_rows, "int32")
     a._keep = (logits, out, choice, tokens, token_offsets, prompt_lens, repetition, frequency, presence,  # noqa: SLF001
                bias_tokens, bias_values, bias_offsets, mask, mask_rows)
+    a._device = _device_of(*a._keep)  # noqa: SLF001
     return a
 
 
 def process_logits(args: LogitsArgs, stream=None) -> None:
     """tqk_process_logits: penalties, biases and masks on the next token's logits, and the greedy choice."""
+    _on_device(args._device)  # noqa: SLF001
     check(tqk_process_logits(ctypes.byref(args), _stream(stream)), "tqk_process_logits")
 
 

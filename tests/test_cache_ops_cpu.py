@@ -131,6 +131,33 @@ def test_python_helpers_refuse_wrong_types(tqk):
         tqk.logits_args(torch.zeros(2, 3, dtype=torch.bfloat16))
 
 
+class _FakeTensor:
+    """What the helpers look at of a CUDA tensor, without a GPU."""
+
+    def __init__(self, device, dtype="float32"):
+        self.device, self.dtype, self.is_cuda = type("D", (), {"index": device}), f"torch.{dtype}", True
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return FAKE
+
+
+def test_python_helpers_refuse_tensors_of_another_device(tqk, monkeypatch):
+    """The library launches on the current device; a call's tensors must share it."""
+    import torch
+    with pytest.raises(ValueError, match="several devices"):
+        tqk.weights_args(_FakeTensor(0), _FakeTensor(1))
+    w = tqk.weights_args(_FakeTensor(1))
+    e = tqk.evict_args(_FakeTensor(1), _FakeTensor(1), 1, 32, 4, 2, weight=_FakeTensor(1))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="cuda:1"):
+        tqk.decode_weights(tqk.DecodeArgs(), w)
+    with pytest.raises(ValueError, match="cuda:1"):
+        tqk.evict(e)
+
+
 def test_plain_eviction():
     """The plain implementation on a case worked out by hand."""
     w = np.array([5, 1, 4, np.nan, 3, 3, 0.5, 9], np.float32)
