@@ -560,9 +560,10 @@ extern "C" int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream)
     p.mask_rows = a->mask_rows;
     p.n_mask_rows = a->n_mask_rows;
     p.err = device_info()->err_word;
-    // CTAs per row: 8, each with at least 2048 tokens, or 16 while all of them run at once (4 per SM).  128256 tokens
-    // with everything on, 16 against 8 CTAs per row: 1 row 9.4 and 14.0 us, 64 rows 39.8 and 30.3 us, 256 rows 168 and 142 us
-    const int most = (long long)a->n_rows * LG_CLUSTER <= 4LL * device_info()->sm_count ? LG_CLUSTER : 8;
+    // CTAs per row: 8, each with at least 2048 tokens, or 16 while all of them run at once (a GPC does not fill up with
+    // clusters of 16, so 3 per SM).  128256 tokens, histories of up to 4000, everything on, 16 against 8 CTAs per row:
+    // 1 row 11.9 and 14.9 us, 24 rows 15.9 and 17.2 us, 37 rows 26.5 and 23.2 us, 256 rows 134 and 95 us (4: 117 us)
+    const int most = (long long)a->n_rows * LG_CLUSTER <= 3LL * device_info()->sm_count ? LG_CLUSTER : 8;
     while (1 << p.log_c < most && a->vocab_size > 2048 << p.log_c) p.log_c++;
     const int cluster = 1 << p.log_c;
     p.own_blocks = (int)(((int64_t)a->vocab_size + (int64_t)cluster * LG_BLOCK - 1) / ((int64_t)cluster * LG_BLOCK));
