@@ -445,7 +445,8 @@ TQK_API int tqk_forward_token(const tqk_model *m, int token, int pos, void *scra
  *   - Histories and bias lists are packed: row r's are entries offsets[r] ..
  *     offsets[r + 1] - 1.  Entries outside [0, vocab_size) are skipped; an offset
  *     outside [0, n_tokens] / [0, n_bias], or falling, is clamped and reported as
- *     TQK_EDEVLEN.  prompt_lens is clamped to the history's length.
+ *     TQK_EDEVLEN.  prompt_lens is clamped to the history's length.  Each entry of a
+ *     bias list whose token the list has more than once is searched for in that list.
  *   - mask: word t / 32, bit t % 32 allows token t.  mask_rows[r] is the mask row
  *     of row r, -1 for no mask; an index from n_mask_rows on (or below -1) allows
  *     nothing and is reported as TQK_EDEVLEN.

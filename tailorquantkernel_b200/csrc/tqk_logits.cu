@@ -17,7 +17,7 @@
 //     branches of the penalties cost by the distinct tokens of the history, not by
 //     the vocabulary;
 //   * each CTA pushes its candidate for the greedy choice to the first CTA's
-//     shared memory and leaves.
+//     shared memory; a cluster barrier later the first CTA compares them.
 #include "tqk_internal.h"
 
 #include <climits>
@@ -395,20 +395,12 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
     extern __shared__ __align__(16) uint32_t counts[];  // p.count_bytes, then the bitmap, then the list
     __shared__ Best warp_best[LG_THREADS / 32];
     __shared__ __align__(8) Best candidate[LG_CLUSTER];  // in the first CTA: every CTA's
-    __shared__ __align__(8) uint64_t pushed;
     const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x, row = blockIdx.y;
     const bool push = p.choice && C > 1;
     if (COUNT) {
         for (int i = tid; i < zero_units(p); i += LG_THREADS) reinterpret_cast<uint4 *>(counts)[i] = uint4{0, 0, 0, 0};
     }
-    if (push) {  // the barrier for the candidates, set up before any CTA can arrive on it
-        if (rank == 0 && tid == 0) {
-            mbar_init(&pushed, (uint32_t)(C - 1));
-            fence_barrier_init();
-        }
-        __syncwarp();
-        cluster_arrive();
-    }
+    if (push) cluster_arrive();
     grid_dependency_wait();
     grid_dependents_launch();
 
@@ -446,23 +438,23 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
         best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.token, o)});
     if ((tid & 31) == 0) warp_best[tid >> 5] = best;
     __syncthreads();
-    if (push) cluster_wait();  // the first CTA's barrier is set up
-    if (tid >= 32) return;
-    best = tid < LG_THREADS / 32 ? warp_best[tid] : Best{-INFINITY, -1};
+    if (push) cluster_wait();  // the first CTA runs, so its shared memory can be written
+    if (tid < 32) {
+        best = tid < LG_THREADS / 32 ? warp_best[tid] : Best{-INFINITY, -1};
 #pragma unroll
-    for (int o = LG_THREADS / 64; o > 0; o >>= 1)
-        best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.token, o)});
-    if (C > 1 && rank != 0) {
-        if (tid == 0) {
+        for (int o = LG_THREADS / 64; o > 0; o >>= 1)
+            best = better(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.token, o)});
+        if (push && rank != 0 && tid == 0)
             st_cluster_u32x2(cluster_map(&candidate[rank], 0), __float_as_uint(best.v), (uint32_t)best.token);
-            mbar_arrive_remote(cluster_map(&pushed, 0));
-        }
-        return;
     }
-    if (C > 1) {
-        // 1 s: the other CTAs of the cluster are resident and only stream their ranges
-        const bool ok = mbar_wait_cluster_bounded(&pushed, 0, 1000000000ull, p.err);
-        if (!__all_sync(0xffffffffu, ok)) return;
+    if (push) {
+        // the first CTA must outlast the last push, however long another CTA's share of the lists takes: a barrier of
+        // the cluster, not a wait with a time limit
+        __syncwarp();
+        cluster_sync_all();
+    }
+    if (rank != 0 || tid >= 32) return;
+    if (push) {
         if (tid > 0) best = tid < C ? candidate[tid] : Best{-INFINITY, -1};
 #pragma unroll
         for (int o = LG_CLUSTER / 2; o > 0; o >>= 1)

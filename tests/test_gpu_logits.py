@@ -241,3 +241,24 @@ def test_histories_at_any_address(tqk, cuda):
         for r in range(rows):
             ref, best = logits_ref(x[r], tokens=ids[off[r]:off[r + 1]], repetition=rep[r])
             assert np.array_equal(out[r].cpu().numpy(), ref) and choice[r].item() == best
+
+
+def test_one_cta_has_all_the_work(tqk, cuda):
+    """A bias list whose tokens all lie in every 16th block of 128 of the vocabulary (one CTA's share, with 16 to a row),
+    each twice and far apart: its search of the list outlasts the other CTAs' work many times over."""
+    import torch
+    rng = np.random.default_rng(8)
+    vocab, rows = 131072, 2
+    x = rng.standard_normal((rows, vocab), dtype=np.float32)
+    own = np.concatenate([np.arange(b, b + 128) for b in range(128, vocab, 16 * 128)]).astype(np.int32)
+    ids = np.tile(np.concatenate([own, rng.permutation(own)]), rows)
+    val = rng.standard_normal(ids.size, dtype=np.float32)
+    val[len(own) + 5] = 100.0  # the first row's choice is among them; the second's may not be
+    off = np.array([0, 2 * len(own), 4 * len(own)], np.int32)
+    out, choice = torch.empty((rows, vocab), device="cuda"), torch.empty(rows, dtype=torch.int32, device="cuda")
+    tqk.process_logits(tqk.logits_args(torch.from_numpy(x).cuda(), out=out, choice=choice, n_bias=ids.size,
+                                       bias_tokens=torch.from_numpy(ids).cuda(), bias_values=torch.from_numpy(val).cuda(),
+                                       bias_offsets=torch.from_numpy(off).cuda()))
+    for r in range(rows):
+        ref, best = logits_ref(x[r], bias=list(zip(ids[off[r]:off[r + 1]].tolist(), val[off[r]:off[r + 1]])))
+        assert np.array_equal(out[r].cpu().numpy(), ref) and choice[r].item() == best
