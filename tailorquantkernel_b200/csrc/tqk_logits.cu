@@ -13,15 +13,18 @@
 //     does not show) and marks them in a bitmap.  Frequent tokens have neighbouring
 //     ids in many vocabularies; dealing out small blocks spreads them over the CTAs;
 //   * the stream reads the bitmap like a second mask; each warp then lists its
-//     marked tokens and works the list off with all lanes, so the division and the
-//     branches of the penalties cost by the distinct tokens of the history, not by
-//     the vocabulary;
+//     marked tokens, fetches their logits again (ahead of the next logits of the
+//     stream, or they would queue behind those: 256 rows 137 us with loads where they
+//     are used, 130 us so) and works the list off with all lanes, so the division and
+//     the branches of the penalties cost by the distinct tokens of the history, not
+//     by the vocabulary;
 //   * each CTA pushes its candidate for the greedy choice to the first CTA's
 //     shared memory; a cluster barrier later the first CTA compares them.
 #include "tqk_internal.h"
 
 #include <climits>
 #include <mutex>
+#include <type_traits>
 
 namespace tqk {
 namespace {
@@ -34,8 +37,9 @@ constexpr int LG_CHUNK = LG_WARPS * LG_LOADS * LG_BLOCK; // 8192 tokens
 constexpr int LG_CLUSTER = 16;                           // most CTAs per row (non-portable above 8), a power of two
 constexpr int LG_COUNT_BYTES_MAX = 64 << 10;             // counters per CTA
 constexpr int LG_LIST = 256;                             // listed tokens per warp at a time
-constexpr int LG_STAGE = LG_WARPS * LG_LIST;             // history entries staged at a time, beside the lists
-constexpr int LG_SCAN = LG_STAGE / LG_THREADS / 4;       // ... 16-byte copies per thread
+constexpr int LG_SCAN = 4 * LG_THREADS;                  // history entries staged at a time: a 16-byte copy per thread
+constexpr int LG_STAGE = 2 * LG_SCAN;                    // ... and the next ones; later the listed tokens' logits
+static_assert(LG_STAGE == LG_WARPS * LG_LIST && LG_LIST >= 2 * LG_BLOCK, "lists and staging share their memory");
 // Counters: 16 bits per token (two to a word) for histories with up to LG_SHORT entries behind the prompt, else 32 bits.
 // From the top: seen, in the bias list, more than once in the bias list, and the count after the prompt.  The width is
 // a value of the row, not of the type: two copies of the row's work in one kernel miss the instruction cache (256 rows
@@ -128,8 +132,8 @@ __device__ __forceinline__ float constrained(const LogitsParams &p, const Row &r
 }
 
 // The CTA's tokens: block b of the row is block b >> log_c of CTA b mod C.  The row's token at place i of them:
-__device__ __forceinline__ int token_at(const LogitsParams &p, int i) {
-    return (((i / LG_BLOCK) << p.log_c) + (int)blockIdx.x) * LG_BLOCK + i % LG_BLOCK;
+__device__ __forceinline__ int token_at(const LogitsParams &p, unsigned i) {
+    return (int)((((i / LG_BLOCK) << p.log_c) + blockIdx.x) * LG_BLOCK + i % LG_BLOCK);
 }
 // ... and the place of token `tok`, or -1 when it is another CTA's or outside the vocabulary.
 __device__ __forceinline__ int place_of(const LogitsParams &p, int tok) {
@@ -186,58 +190,78 @@ __device__ __forceinline__ uint32_t lane_bits(uint32_t words, int k) {
     return bits;
 }
 
-// Counts the history's entries among this CTA's tokens [c0, c0 + span) and marks them in the bitmap.  The entries are
-// staged in shared memory, 2048 at a time, so that they take no registers beside the logits; each warp picks the
-// CTA's (one in C) out of its 256 and then counts those with all lanes.
+// Adds unit to (ADD) or sets it in a word of shared memory and sets a bit in another, without a branch.
+template <bool ADD>
+__device__ __forceinline__ void mark_shared(bool go, uint32_t word, uint32_t unit, uint32_t bits, uint32_t bit) {
+    if constexpr (ADD)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %0, 0;\n\t@p red.shared.add.u32 [%1], %2;\n\t"
+                     "@p red.shared.or.b32 [%3], %4;\n\t}" ::"r"((uint32_t)go), "r"(word), "r"(unit), "r"(bits), "r"(bit)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %0, 0;\n\t@p red.shared.or.b32 [%1], %2;\n\t"
+                     "@p red.shared.or.b32 [%3], %4;\n\t}" ::"r"((uint32_t)go), "r"(word), "r"(unit), "r"(bits), "r"(bit)
+                     : "memory");
+}
+
+// Counts the history's entries among this CTA's tokens [c0, c0 + span) and marks them in the bitmap, once the CTA's
+// threads have met (the counters are zero then).  The entries are staged in shared memory, 1024 at a time and the next
+// 1024 on their way, so that they take no registers beside the logits.  What bounds this is the instructions issued,
+// every CTA of the row looking at every entry (256 rows: 68 M warp instructions, 16 M without histories): each lane
+// updates its own entries, one in C active, without a branch.  Collecting the CTA's entries first, to update them with
+// all lanes, takes more of them (256 rows 130 us, 121 us so).
 __device__ __forceinline__ void count_history(const LogitsParams &p, const Row &r, int c0, uint32_t *bitmap, uint32_t *lists) {
     const Counters &k = r.counters;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    uint32_t *staged = lists + LG_WARPS * LG_LIST, *picked = lists + warp * LG_LIST;  // tokens, bit 31: generated
-    const uint32_t below = (1u << lane) - 1, deal = (1u << p.log_c) - 1;
+    const int tid = threadIdx.x;
+    const uint32_t staged = smem_u32(lists + LG_WARPS * LG_LIST + 4 * tid);  // this thread's
     // from a 16-byte boundary on; entries before h0 are skipped.  An array that is not 16-byte aligned is copied word by word
-    const bool wide = (reinterpret_cast<uintptr_t>(p.tokens) & 15) == 0;
+    const int wide_end = (reinterpret_cast<uintptr_t>(p.tokens) & 15) == 0 ? min(p.n_tokens - 3, r.h1) : INT_MIN;
+    auto fetch = [&](int base, uint32_t to) {
+        const int i = base + 4 * tid;
+        if (i < wide_end) copy_async_16(to, p.tokens + i);
+        else
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < r.h1) copy_async_4(to + 4 * j, p.tokens + i + j);
+        copy_async_commit();
+    };
+    // a token's block is the CTA's when the block's last bits are its rank; the CTA's places below `end` are in the span
+    // and in the vocabulary
+    const uint32_t rank = blockIdx.x * LG_BLOCK, deal = ((1u << p.log_c) - 1) * LG_BLOCK;
+    const int last = (p.vocab - 1) / LG_BLOCK, blocks = (last - (int)blockIdx.x + (1 << p.log_c)) >> p.log_c;
+    const bool last_own = ((last * LG_BLOCK) & (int)deal) == (int)rank;
+    const int end = min(max(blocks * LG_BLOCK - (last_own ? (last + 1) * LG_BLOCK - p.vocab : 0) - c0, 0), r.span);
+    const uint32_t words = smem_u32(k.words), bits = smem_u32(bitmap), seen = k.seen(), to_bytes = 2 - k.half;
+    // the entries at base .. base + LG_SCAN - 1 that lie in [from, to), this thread's in v
+    auto count = [&](uint4 v, int base, int from, int to, auto made) {
+        uint32_t tok[4] = {v.x, v.y, v.z, v.w};
+        if (base < from || base + LG_SCAN > to) {
+            const int i = base + 4 * tid;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < from || i + j >= to) tok[j] = UINT_MAX;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t t = (((tok[j] >> p.log_c) & ~(LG_BLOCK - 1u)) | (tok[j] & (LG_BLOCK - 1u))) - c0;
+            const uint32_t word = words + ((t << to_bytes) & ~3u), unit = (decltype(made)::value ? 1u : seen) << k.shift(t);
+            mark_shared<decltype(made)::value>(((tok[j] ^ rank) & deal) == 0 && t < (uint32_t)end, word, unit,
+                                               bits + (t >> 5) * 4, __funnelshift_l(0u, 1u, t));
+        }
+    };
+    const int first = r.h0 & ~3;
+    fetch(first, staged);
+    fetch(first + LG_SCAN, staged + LG_SCAN * 4);
+    __syncthreads();
+    uint32_t turn = 0;
 #pragma unroll 1
-    for (int base = r.h0 & ~3; base < r.h1; base += LG_STAGE) {
-#pragma unroll
-        for (int q = 0; q < LG_SCAN; q++) {
-            const int e = 4 * (q * LG_THREADS + tid), i = base + e;
-            if (wide && i + 4 <= p.n_tokens) {
-                if (i < r.h1) copy_async_16(staged + e, p.tokens + i);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (i + j < r.h1) copy_async_4(staged + e + j, p.tokens + i + j);
-            }
-        }
-        copy_async_wait_all();  // each thread reads only what it copied
-        int n = 0;
-#pragma unroll
-        for (int q = 0; q < LG_SCAN; q++) {
-            const int e = 4 * (q * LG_THREADS + tid), i = base + e;
-            const uint4 v = *reinterpret_cast<const uint4 *>(staged + e);
-            const uint32_t tok[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool mine = ((tok[j] / LG_BLOCK) & deal) == blockIdx.x && tok[j] < (uint32_t)p.vocab &&
-                                  i + j >= r.h0 && i + j < r.h1;
-                const uint32_t lanes = __ballot_sync(0xffffffffu, mine);
-                if (mine) picked[n + __popc(lanes & below)] = tok[j] | (i + j >= r.prompt_end ? 0x80000000u : 0u);
-                n += __popc(lanes);
-            }
-        }
-        __syncwarp();
-        for (int q = lane; q < n; q += 32) {
-            const uint32_t e = picked[q], tok = e & 0x7FFFFFFFu;
-            const int t = (int)((tok / LG_BLOCK) >> p.log_c) * LG_BLOCK + (int)(tok % LG_BLOCK) - c0;
-            if ((unsigned)t >= (unsigned)r.span) continue;
-            // frequent tokens meet here again and again: a flag that is set already needs no atomic
-            const uint32_t flag = k.seen() << k.shift(t), bit = 1u << (t & 31);
-            if (e >> 31) atomicAdd(k.word(t), 1u << k.shift(t));
-            else if (!(*k.word(t) & flag)) atomicOr(k.word(t), flag);
-            if (!(bitmap[t >> 5] & bit)) atomicOr(&bitmap[t >> 5], bit);
-        }
-        __syncwarp();
+    for (int base = first; base < r.h1; base += LG_SCAN, turn ^= LG_SCAN * 4) {
+        copy_async_wait<1>();  // each thread reads only what it copied
+        const uint4 v = ld_shared_u32x4(staged + turn);
+        fetch(base + 2 * LG_SCAN, staged + turn);
+        if (base < r.prompt_end) count(v, base, r.h0, r.prompt_end, std::false_type{});
+        if (base + LG_SCAN > r.prompt_end && r.prompt_end < r.h1) count(v, base, r.prompt_end, r.h1, std::true_type{});
     }
+    copy_async_wait_all();
 }
 
 // This CTA's share of a row.  On entry x holds the first chunk, and the counters and their bitmap are zero.
@@ -249,39 +273,50 @@ __device__ __forceinline__ Best work_row(const LogitsParams &p, const Row &r, ui
     const int own = p.own_blocks * LG_BLOCK, step = (LG_WARPS << p.log_c) * LG_BLOCK;
     Best top{-INFINITY, -1};   // of the warp's streamed tokens
     Best best{-INFINITY, -1};  // of this thread's listed ones
-    uint16_t *list = reinterpret_cast<uint16_t *>(lists + warp * LG_LIST);  // this warp's: bits of its words, 32 w + b
+    // this warp's marked tokens as bits of its words, 32 w + b, and their logits
+    uint16_t *list = reinterpret_cast<uint16_t *>(lists + warp * LG_LIST);
+    float *list_v = reinterpret_cast<float *>(lists + (LG_WARPS + warp) * LG_LIST);
     uint32_t words = load_words(p, r, 0);
     int c0 = 0;
     auto settle = [&](int t, float v) {
         if (v > best.v || (v == best.v && best.token >= 0 && t < best.token)) best = Best{v, t};
         if (r.dst) r.dst[t] = v;
     };
-    // the warp's marked tokens of the chunk at t0, `mask` its mask words; those with a bias are left to the bias list
-    auto work_off = [&](uint32_t marks, uint32_t mask, int t0) {
-        while (__any_sync(0xffffffffu, marks != 0)) {  // once, unless there are more than the list holds
-            int at = __popc(marks);
-            if (__reduce_add_sync(0xffffffffu, at) > LG_LIST) at = min(at, LG_LIST / 32);
-            const int n_own = at;
+    // lists marked tokens of the chunk at t0, as many as fit, and takes them out of marks; their logits are on their way
+    auto list_marks = [&](uint32_t &marks, int t0) {
+        if (!__any_sync(0xffffffffu, marks)) return 0;
+        int at = __popc(marks);
+        if (__reduce_add_sync(0xffffffffu, at) > LG_LIST) at = min(at, LG_LIST / 32);
+        const int n_own = at;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, at, o);
-                if (lane >= o) at += x;
-            }
-            const int n = __shfl_sync(0xffffffffu, at, 31);
-            at -= n_own;
-            for (int q = 0; q < n_own; q++, marks &= marks - 1) list[at + q] = (uint16_t)(32 * lane + __ffs(marks) - 1);
-            __syncwarp();
-            for (int q0 = 0; q0 < n; q0 += 32) {
-                const int e = q0 + lane < n ? list[q0 + lane] : 0;
-                const bool allowed = (__shfl_sync(0xffffffffu, mask, e >> 5) >> (e & 31)) & 1u;
-                if (q0 + lane >= n) continue;
-                const int i = t0 + (warp + (e >> 7) * LG_WARPS) * LG_BLOCK + e % LG_BLOCK, t = token_at(p, i);
-                const float v = __ldcg(r.src + t);  // in place: still the logit
-                const uint32_t c = counters.get(i - c0);
-                if (!(c & counters.biased())) settle(t, allowed ? constrained(p, r, v, c, 0.0f) : -INFINITY);
-            }
-            __syncwarp();
+        for (int o = 1; o < 32; o <<= 1) {
+            const int before = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += before;
         }
+        const int n = __shfl_sync(0xffffffffu, at, 31);
+        at -= n_own;
+        const float *from = r.src + token_at(p, t0 + (warp + (lane >> 2) * LG_WARPS) * LG_BLOCK) + 32 * (lane & 3);
+        for (int q = 0; q < n_own; q++, marks &= marks - 1) {
+            const int b = __ffs(marks) - 1;
+            list[at + q] = (uint16_t)(32 * lane + b);
+            copy_async_4(smem_u32(list_v + at + q), from + b);  // in place: still the logit
+        }
+        return n;
+    };
+    // the n listed tokens of the chunk at t0, `mask` its mask words; those with a bias are left to the bias list
+    auto work_off = [&](int n, uint32_t mask, int t0) {
+        copy_async_wait_all();
+        __syncwarp();
+        for (int q0 = 0; q0 < n; q0 += 32) {
+            const unsigned e = q0 + lane < n ? list[q0 + lane] : 0;
+            const bool allowed = (__shfl_sync(0xffffffffu, mask, e >> 5) >> (e & 31)) & 1u;
+            if (q0 + lane >= n) continue;
+            const unsigned i = t0 + (warp + e / LG_BLOCK * LG_WARPS) * LG_BLOCK + e % LG_BLOCK;
+            const uint32_t c = counters.get(i - c0);
+            if (!(c & counters.biased()))
+                settle(token_at(p, i), allowed ? constrained(p, r, list_v[q0 + lane], c, 0.0f) : -INFINITY);
+        }
+        __syncwarp();
     };
     for (int t0 = 0; t0 < own; t0 += LG_CHUNK) {
         if constexpr (COUNT) {
@@ -293,7 +328,6 @@ __device__ __forceinline__ Best work_row(const LogitsParams &p, const Row &r, ui
                         reinterpret_cast<uint4 *>(counters.words)[i] = uint4{0, 0, 0, 0};
                 }
                 c0 = t0;
-                __syncthreads();
                 count_history(p, r, c0, bitmap, lists);
                 for (int i = r.b0 + tid; i < r.b1; i += LG_THREADS) {
                     const int t = place_of(p, p.bias_tokens[i]) - c0;
@@ -357,13 +391,20 @@ __device__ __forceinline__ Best work_row(const LogitsParams &p, const Row &r, ui
             }
         }
         const uint32_t mask = words;
+        int n_listed = 0;
+        if constexpr (COUNT) {
+            __syncwarp();
+            n_listed = list_marks(marks, t0);
+        }
         if (t0 + LG_CHUNK < own) {  // the next logits load while the marked tokens are worked off
             load_chunk<VEC>(p, r.src, t0 + LG_CHUNK, x);
             words = load_words(p, r, t0 + LG_CHUNK);
         }
         if constexpr (COUNT) {
-            __syncwarp();
-            work_off(marks, mask, t0);
+            while (n_listed > 0) {  // once, unless there are more than the list holds
+                work_off(n_listed, mask, t0);
+                n_listed = list_marks(marks, t0);
+            }
             // ---- the span's tokens with a bias, once their raw logits are stored
             if (r.b1 > r.b0 && (t0 + LG_CHUNK >= own || t0 + LG_CHUNK == c0 + r.span)) {
                 __syncthreads();
@@ -554,7 +595,7 @@ extern "C" int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream)
     p.err = device_info()->err_word;
     // CTAs per row: 8, each with at least 2048 tokens, or 16 while all of them run at once (a GPC does not fill up with
     // clusters of 16, so 3 per SM).  128256 tokens, histories of up to 4000, everything on, 16 against 8 CTAs per row:
-    // 1 row 11.9 and 14.9 us, 24 rows 15.9 and 17.2 us, 37 rows 26.5 and 23.2 us, 256 rows 134 and 95 us (4: 117 us)
+    // 1 row 11.2 and 13.8 us, 24 rows 16.1 and 16.2 us, 37 rows 25.5 and 22.4 us, 256 rows 129 and 93 us (4: 103 us)
     const int most = (long long)a->n_rows * LG_CLUSTER <= 3LL * device_info()->sm_count ? LG_CLUSTER : 8;
     while (1 << p.log_c < most && a->vocab_size > 2048 << p.log_c) p.log_c++;
     const int cluster = 1 << p.log_c;
