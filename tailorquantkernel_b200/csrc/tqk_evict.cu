@@ -8,8 +8,8 @@
 // not have to: about budget * (n - budget) / n rows of a cache cut to `budget`,
 // one row of a cache that is one row over.
 //
-// One thread-block cluster per (item, kv head), a contiguous part of the slots
-// per CTA:
+// One thread-block cluster per (item, kv head) -- several where SMs are left
+// over, which share step 4 -- a contiguous part of the slots per CTA:
 //   1. keys: the rank of a row as 32 bits that compare unsigned (protected rows
 //      above every weight), into shared memory;
 //   2. the budget-th largest key by radix select, 11 + 11 + 10 bits: a histogram
@@ -43,6 +43,8 @@ constexpr int EV_LOADS = 8;                     // sums and positions in flight 
 constexpr int EV_ALONE = 100 << 10;             // dynamic shared memory that leaves no room for a second CTA
 constexpr int EV_KEY_BYTES_MAX = 140 << 10;     // dynamic shared memory at the longest length
 constexpr int EV_NARROW = 1024;                 // slots per CTA where every CTA has an SM
+constexpr int EV_PARTS_MAX = 8;                 // clusters per (item, kv head)
+constexpr int EV_PARTS_MOVES = 4096;            // from so many moves on
 constexpr int EV_STAGE = 8192;                  // slots per CTA whose positions are staged in shared memory
 static_assert(EV_CLUSTER_MAX * EV_THREADS * EV_RUN_MAX == TQK_EVICT_MAX_LEN, "documented limit");
 
@@ -142,11 +144,14 @@ __device__ __forceinline__ void move_rows(uint8_t *kh, uint8_t *vh, int src, int
     }
 }
 
-template <int NB, int T>
+// PARTS: several clusters share an (item, kv head)'s moves.
+template <int NB, int T, bool PARTS>
 __global__ void __launch_bounds__(T, 1024 / T) evict_kernel(const EvictParams p) {
     extern __shared__ __align__(16) uint32_t keys[];  // [T * run], then the slots of holes and movers
     __shared__ EvictShared<T> sh;
-    const int tid = threadIdx.x, C = (int)gridDim.x, rank = (int)blockIdx.x;
+    const int tid = threadIdx.x, C = PARTS ? EV_CLUSTER_MAX : (int)gridDim.x;
+    const int rank = PARTS ? (int)blockIdx.x % EV_CLUSTER_MAX : (int)blockIdx.x;
+    const int part = PARTS ? (int)blockIdx.x / EV_CLUSTER_MAX : 0, parts = PARTS ? (int)gridDim.x / EV_CLUSTER_MAX : 1;
     for (int i = tid; i < 3 * EV_BINS / 4; i += T) reinterpret_cast<uint4 *>(sh.hist)[i] = uint4{0, 0, 0, 0};
     if (tid == 0) {
         sh.max_pos = INT_MIN;
@@ -162,13 +167,13 @@ __global__ void __launch_bounds__(T, 1024 / T) evict_kernel(const EvictParams p)
         len = len < 0 ? 0 : p.len_cap;
     }
     const int budget = p.budget;
-    if (p.lens_out && rank == 0 && kvh == 0 && tid == 0) p.lens_out[item] = min(len, budget);
+    if (p.lens_out && blockIdx.x == 0 && kvh == 0 && tid == 0) p.lens_out[item] = min(len, budget);
     const long long at = (long long)item * p.stat_stride + (long long)kvh * p.max_tokens;
     const float *w_in = p.weight + at;
     float *w_out = p.weight_out + at;
     const int *pos_in = p.position ? p.position + at : nullptr;
     int *pos_out = p.position ? p.position_out + at : nullptr;
-    const bool copy_w = w_out != w_in, copy_pos = pos_out != pos_in;
+    const bool copy_w = part == 0 && w_out != w_in, copy_pos = part == 0 && pos_out != pos_in;
     // this CTA's slots [s0, s1), `run` consecutive ones per thread; an odd run keeps the threads' shared-memory
     // words in different banks
     const int run = ((len + C * T - 1) / (C * T)) | 1;
@@ -365,6 +370,8 @@ __global__ void __launch_bounds__(T, 1024 / T) evict_kernel(const EvictParams p)
     if (tid == 0 && sh.pre_m[C] != sh.pre_h[C]) record_error(p.err, DEVERR_BADLEN);
     const long long n_moves = sh.pre_m[C] == sh.pre_h[C] ? sh.pre_m[C] : 0;
     const int m0 = (int)(n_moves * rank / C), m1 = (int)(n_moves * (rank + 1) / C);
+    // of them this part's rows
+    const int k0 = m0 + (int)((long long)(m1 - m0) * part / parts), k1 = m0 + (int)((long long)(m1 - m0) * (part + 1) / parts);
     const long long head_off = (long long)item * p.item_stride + (long long)kvh * p.max_tokens * (NB * BLOCK_BYTES);
     // up to 32 moves at a time per warp, a lane looking each of them up
     auto slot_of = [&](const int *pre, int j, bool mover) {
@@ -372,19 +379,25 @@ __global__ void __launch_bounds__(T, 1024 / T) evict_kernel(const EvictParams p)
         while (r + 1 < C && pre[r + 1] <= j) r++;
         return (int)ld_cluster_u32(cluster_map(mover ? &list[last - (j - pre[r])] : &list[j - pre[r]], (uint32_t)r));
     };
+    auto move_stats = [&](int src, int dst) {
+        w_out[dst] = w_in[src];
+        if (pos_in) pos_out[dst] = pos_in[src];
+    };
     // few moves are spread over the warps
-    const int lane = tid & 31, step = max(1, min(32, (m1 - m0 + (T / 32) - 1) / (T / 32)));
-    for (int b = m0 + (tid >> 5) * step; b < m1; b += (T / 32) * step) {
-        const int n = min(step, m1 - b);
+    const int lane = tid & 31, step = max(1, min(32, (k1 - k0 + (T / 32) - 1) / (T / 32)));
+    for (int b = k0 + (tid >> 5) * step; b < k1; b += (T / 32) * step) {
+        const int n = min(step, k1 - b);
         int src = 0, dst = 0;
         if (lane < n) {
             src = slot_of(sh.pre_m, b + lane, true);
             dst = slot_of(sh.pre_h, b + lane, false);
-            w_out[dst] = w_in[src];
-            if (pos_in) pos_out[dst] = pos_in[src];
+            if (part == 0) move_stats(src, dst);
         }
         move_rows<NB>(p.k + head_off, p.v + head_off, src, dst, n);
     }
+    // the sums and positions of the other parts' rows: written by the part that copied the rest of them
+    if (PARTS && part == 0)
+        for (int j = k1 + tid; j < m1; j += T) move_stats(slot_of(sh.pre_m, j, true), slot_of(sh.pre_h, j, false));
     if (C > 1) cluster_barrier();  // no CTA leaves while another reads its list
 }
 
@@ -396,7 +409,7 @@ __global__ void evict_lens_kernel(const int *lens, int len0, int len_step, int l
     if (i < n) out[i] = min(min(max(lens ? lens[i] : len0 + i * len_step, 0), len_cap), budget);
 }
 
-template <int NB, int T>
+template <int NB, int T, bool PARTS>
 int launch_evict(const EvictParams &p, int cluster, dim3 grid, cudaStream_t stream) {
     size_t smem = (size_t)T * p.run * (p.staged ? 2 : 1) * sizeof(uint32_t);
     // few CTAs: one per SM (two would share an SM while others idle)
@@ -410,23 +423,23 @@ int launch_evict(const EvictParams &p, int cluster, dim3 grid, cudaStream_t stre
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[dev]) {
-            e = cudaFuncSetAttribute(evict_kernel<NB, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(evict_kernel<NB, T, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      EV_KEY_BYTES_MAX);
             if (e != cudaSuccess) return fail_cuda(e, "tqk_evict_q8: kernel attributes");
             ready[dev] = true;
         }
     }
-    if (cluster == 1) return launch_pdl(evict_kernel<NB, T>, grid, dim3(T), smem, stream, p);
-    return launch_pdl_cluster(evict_kernel<NB, T>, grid, dim3(T), smem, stream, (unsigned)cluster, p);
+    if (cluster == 1) return launch_pdl(evict_kernel<NB, T, PARTS>, grid, dim3(T), smem, stream, p);
+    return launch_pdl_cluster(evict_kernel<NB, T, PARTS>, grid, dim3(T), smem, stream, (unsigned)cluster, p);
 }
 
-template <int T>
+template <int T, bool PARTS>
 int dispatch_evict(int nb, const EvictParams &p, int cluster, dim3 grid, cudaStream_t stream) {
     switch (nb) {
-        case 1: return launch_evict<1, T>(p, cluster, grid, stream);
-        case 2: return launch_evict<2, T>(p, cluster, grid, stream);
-        case 4: return launch_evict<4, T>(p, cluster, grid, stream);
-        default: return launch_evict<8, T>(p, cluster, grid, stream);
+        case 1: return launch_evict<1, T, PARTS>(p, cluster, grid, stream);
+        case 2: return launch_evict<2, T, PARTS>(p, cluster, grid, stream);
+        case 4: return launch_evict<4, T, PARTS>(p, cluster, grid, stream);
+        default: return launch_evict<8, T, PARTS>(p, cluster, grid, stream);
     }
 }
 
@@ -507,13 +520,26 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
         const long long units = (long long)a->n_items * a->n_kv_heads;
         while (cluster < EV_CLUSTER_MAX && cluster * EV_NARROW < max_len && 2 * cluster * units <= device_info()->sm_count)
             cluster *= 2;
-        const dim3 grid((unsigned)cluster, (unsigned)a->n_kv_heads, (unsigned)a->n_items);
+        // Moving many rows keeps the SMs that do it busy for longer than finding them.  Where SMs are left over and the
+        // sums and positions go elsewhere (a cluster may still read them when another is done), several clusters share
+        // a head's moves, each finding them for itself.  Half of 131072 rows kept, with one cluster per head and so: 1
+        // head 66 and 33 us, 2 heads 69 and 46 us, 4 heads 72 and 60 us.  Only up to half of the SMs: 16 clusters of 8
+        // do not all run at once (8 heads: 85 and 123 us; 8 clusters of 16 CTAs do not either: 112 us)
+        int parts = 1;
+        const long long busy = units * cluster;
+        const int moves = a->budget < max_len - a->budget ? a->budget : max_len - a->budget;  // at most, at max_len
+        if (cluster == EV_CLUSTER_MAX && moves >= EV_PARTS_MOVES && a->weight_out != a->weight &&
+            (!a->position || a->position_out != a->position))
+            while (parts < EV_PARTS_MAX && 2 * parts * busy <= device_info()->sm_count / 2) parts *= 2;
+        const dim3 grid((unsigned)(cluster * parts), (unsigned)a->n_kv_heads, (unsigned)a->n_items);
         const bool wide = max_len > EV_STAGE / 2 && (long long)grid.x * grid.y * grid.z <= device_info()->sm_count;
         const int threads = wide ? EV_WIDE : EV_THREADS;
         p.run = ((max_len + cluster * threads - 1) / (cluster * threads)) | 1;
         p.staged = max_len <= cluster * EV_STAGE;
         p.lens_out = a->lens_out != a->lens ? a->lens_out : nullptr;
-        rc = wide ? dispatch_evict<EV_WIDE>(nb, p, cluster, grid, st) : dispatch_evict<EV_THREADS>(nb, p, cluster, grid, st);
+        rc = parts > 1 ? dispatch_evict<EV_WIDE, true>(nb, p, cluster, grid, st)
+             : wide    ? dispatch_evict<EV_WIDE, false>(nb, p, cluster, grid, st)
+                       : dispatch_evict<EV_THREADS, false>(nb, p, cluster, grid, st);
         if (rc) return rc;
     }
     if (!a->lens_out || (max_len > 0 && a->lens_out != a->lens)) return TQK_OK;

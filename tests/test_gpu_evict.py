@@ -126,6 +126,21 @@ def test_evict(tqk, cuda, nkv, hd, mt, lens, device_lens, budget, first, recent,
     assert tqk.device_status() == 0
 
 
+FEW_HEADS = [  # out of place, several clusters share a head's moves
+    (1, 256, 20001, [20001], False, 10000, 4, 100, "normal", "mixed"),
+    (2, 128, 30000, [30000, 17000], True, 12345, 4, 100, "ties", "mixed"),      # the second: fewer moves
+    (1, 128, 30000, [0, 30000, 15000, 15001], True, 15000, 0, 0, "odd", None),  # nothing, all, nothing, one row
+    (4, 64, 9000, [9000], False, 4500, 4, 100, "equal", "rising"),
+    (3, 32, 120000, [120000], False, 4096, 4, 100, "normal", "rising"),
+]
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("nkv,hd,mt,lens,device_lens,budget,first,recent,weights,positions", FEW_HEADS)
+def test_few_heads(tqk, cuda, nkv, hd, mt, lens, device_lens, budget, first, recent, weights, positions, in_place):
+    test_evict(tqk, cuda, nkv, hd, mt, lens, device_lens, budget, first, recent, weights, positions, in_place)
+
+
 def test_lengths_from_the_device_are_clamped(tqk, cuda):
     import torch
     nkv, hd, mt = 1, 32, 50
