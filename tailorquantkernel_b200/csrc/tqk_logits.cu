@@ -39,7 +39,7 @@ constexpr int LG_COUNT_BYTES_MAX = 64 << 10;             // counters per CTA
 constexpr int LG_LIST = 256;                             // listed tokens per warp at a time
 constexpr int LG_SCAN = 4 * LG_THREADS;                  // history entries staged at a time: a 16-byte copy per thread
 constexpr int LG_STAGE = 2 * LG_SCAN;                    // ... and the next ones; later the listed tokens' logits
-static_assert(LG_STAGE == LG_WARPS * LG_LIST && LG_LIST >= 2 * LG_BLOCK, "lists and staging share their memory");
+static_assert(LG_STAGE == LG_WARPS * LG_LIST, "the listed logits take the staging's memory");
 // Counters: 16 bits per token (two to a word) for histories with up to LG_SHORT entries behind the prompt, else 32 bits.
 // From the top: seen, in the bias list, more than once in the bias list, and the count after the prompt.  The width is
 // a value of the row, not of the type: two copies of the row's work in one kernel miss the instruction cache (256 rows
@@ -212,7 +212,7 @@ __device__ __forceinline__ void mark_shared(bool go, uint32_t word, uint32_t uni
 __device__ __forceinline__ void count_history(const LogitsParams &p, const Row &r, int c0, uint32_t *bitmap, uint32_t *lists) {
     const Counters &k = r.counters;
     const int tid = threadIdx.x;
-    const uint32_t staged = smem_u32(lists + LG_WARPS * LG_LIST + 4 * tid);  // this thread's
+    const uint32_t staged = smem_u32(lists + 4 * tid);  // this thread's
     // from a 16-byte boundary on; entries before h0 are skipped.  An array that is not 16-byte aligned is copied word by word
     const int wide_end = (reinterpret_cast<uintptr_t>(p.tokens) & 15) == 0 ? min(p.n_tokens - 3, r.h1) : INT_MIN;
     auto fetch = [&](int base, uint32_t to) {
@@ -274,8 +274,8 @@ __device__ __forceinline__ Best work_row(const LogitsParams &p, const Row &r, ui
     Best top{-INFINITY, -1};   // of the warp's streamed tokens
     Best best{-INFINITY, -1};  // of this thread's listed ones
     // this warp's marked tokens as bits of its words, 32 w + b, and their logits
-    uint16_t *list = reinterpret_cast<uint16_t *>(lists + warp * LG_LIST);
-    float *list_v = reinterpret_cast<float *>(lists + (LG_WARPS + warp) * LG_LIST);
+    uint16_t *list = reinterpret_cast<uint16_t *>(lists + LG_STAGE) + warp * LG_LIST;
+    float *list_v = reinterpret_cast<float *>(lists) + warp * LG_LIST;
     uint32_t words = load_words(p, r, 0);
     int c0 = 0;
     auto settle = [&](int t, float v) {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
     }
     if (COUNT && p.bias_tokens) list_range(p.bias_offsets, row, p.n_bias, p.err, report, r.b0, r.b1);
     uint32_t *bitmap = counts + p.count_bytes / 4;
-    uint32_t *lists = bitmap + p.count_bytes / 64;  // a word per entry while the history is counted
+    uint32_t *lists = bitmap + p.count_bytes / 64;  // LG_STAGE words, then 16 bits per listed token
     r.counters = Counters{counts, r.h1 - r.prompt_end <= LG_SHORT};
     r.span = r.counters.half ? p.count_bytes / 2 : p.count_bytes / 4;
     Best best = work_row<VEC, COUNT>(p, r, bitmap, lists, x);
@@ -504,7 +504,9 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
     if (tid == 0) p.choice[row] = best.token;
 }
 
-size_t logits_smem(int count_bytes) { return count_bytes + count_bytes / 16 + (LG_WARPS * LG_LIST + LG_STAGE) * 4; }
+// What shared memory takes is lost for loads in flight, in steps: 4 CTAs of 47 KB (32 KB of counters) leave 60 KB of L1,
+// 4 CTAs of 51 KB only 28 KB (256 rows of 128256 tokens: 111 and 121 us).
+size_t logits_smem(int count_bytes) { return count_bytes + count_bytes / 16 + LG_STAGE * 4 + LG_WARPS * LG_LIST * 2; }
 
 template <bool VEC, bool COUNT>
 int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
@@ -595,7 +597,7 @@ extern "C" int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream)
     p.err = device_info()->err_word;
     // CTAs per row: 8, each with at least 2048 tokens, or 16 while all of them run at once (a GPC does not fill up with
     // clusters of 16, so 3 per SM).  128256 tokens, histories of up to 4000, everything on, 16 against 8 CTAs per row:
-    // 1 row 11.2 and 13.8 us, 24 rows 16.1 and 16.2 us, 37 rows 25.5 and 22.4 us, 256 rows 129 and 93 us (4: 103 us)
+    // 1 row 10.9 and 13.7 us, 24 rows 15.6 and 15.8 us, 37 rows 24.9 and 21.0 us, 256 rows 126 and 86 us (4: 103 us)
     const int most = (long long)a->n_rows * LG_CLUSTER <= 3LL * device_info()->sm_count ? LG_CLUSTER : 8;
     while (1 << p.log_c < most && a->vocab_size > 2048 << p.log_c) p.log_c++;
     const int cluster = 1 << p.log_c;
