@@ -35,6 +35,7 @@ constexpr int LG_BLOCK = 128;                            // tokens per block: a 
 constexpr int LG_LOADS = 8;                              // blocks per warp and chunk, in registers
 constexpr int LG_CHUNK = LG_WARPS * LG_LOADS * LG_BLOCK; // 8192 tokens
 constexpr int LG_CLUSTER = 16;                           // most CTAs per row (non-portable above 8), a power of two
+constexpr int LG_OWN = 16384;                            // tokens per CTA, from which more CTAs take a row
 constexpr int LG_COUNT_BYTES_MAX = 64 << 10;             // counters per CTA
 constexpr int LG_LIST = 256;                             // listed tokens per warp at a time
 constexpr int LG_SCAN = 4 * LG_THREADS;                  // history entries staged at a time: a 16-byte copy per thread
@@ -80,7 +81,8 @@ struct LogitsParams {
     int n_mask_rows;
     int log_c;        // log2 of the CTAs per row
     int own_blocks;   // blocks per CTA
-    int count_bytes;  // counters' shared memory, whole chunks
+    int count_bytes;  // counters' shared memory
+    int bitmap_bytes; // the bitmap's: whole chunks
     int *err;
 };
 
@@ -102,8 +104,8 @@ __device__ __forceinline__ Best better(Best a, Best b) {
     return take ? b : a;
 }
 
-// 16-byte units of the counters and the bitmap of counted tokens behind them, a bit per 16-bit counter's token.
-__device__ __forceinline__ int zero_units(const LogitsParams &p) { return (p.count_bytes + p.count_bytes / 16) / 16; }
+// 16-byte units of the counters and the bitmap of counted tokens behind them.
+__device__ __forceinline__ int zero_units(const LogitsParams &p) { return (p.count_bytes + p.bitmap_bytes) / 16; }
 
 // What all threads of a CTA know of their row.
 struct Row {
@@ -113,7 +115,7 @@ struct Row {
     bool barred;           // a bad mask row index: nothing is allowed
     int h0, h1, prompt_end, b0, b1;
     Counters counters;
-    int span;  // tokens that the counters cover at a time, whole chunks
+    int span;  // tokens that the counters cover at a time: whole chunks, or all of the CTA's
     float repetition, frequency, presence;
 };
 
@@ -467,9 +469,10 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
     }
     if (COUNT && p.bias_tokens) list_range(p.bias_offsets, row, p.n_bias, p.err, report, r.b0, r.b1);
     uint32_t *bitmap = counts + p.count_bytes / 4;
-    uint32_t *lists = bitmap + p.count_bytes / 64;  // LG_STAGE words, then 16 bits per listed token
+    uint32_t *lists = bitmap + p.bitmap_bytes / 4;  // LG_STAGE words, then 16 bits per listed token
     r.counters = Counters{counts, r.h1 - r.prompt_end <= LG_SHORT};
-    r.span = r.counters.half ? p.count_bytes / 2 : p.count_bytes / 4;
+    const int fit = p.count_bytes / (r.counters.half ? 2 : 4);
+    r.span = fit >= p.own_blocks * LG_BLOCK ? fit : fit / LG_CHUNK * LG_CHUNK;
     Best best = work_row<VEC, COUNT>(p, r, bitmap, lists, x);
 
     // ---- the greedy choice
@@ -506,11 +509,11 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
 
 // What shared memory takes is lost for loads in flight, in steps: 4 CTAs of 47 KB (32 KB of counters) leave 60 KB of L1,
 // 4 CTAs of 51 KB only 28 KB (256 rows of 128256 tokens: 111 and 121 us).
-size_t logits_smem(int count_bytes) { return count_bytes + count_bytes / 16 + LG_STAGE * 4 + LG_WARPS * LG_LIST * 2; }
+size_t logits_smem(int count_bytes, int bitmap_bytes) { return count_bytes + bitmap_bytes + LG_STAGE * 4 + LG_WARPS * LG_LIST * 2; }
 
 template <bool VEC, bool COUNT>
 int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
-    const size_t smem = COUNT ? logits_smem(p.count_bytes) : 0;
+    const size_t smem = COUNT ? logits_smem(p.count_bytes, p.bitmap_bytes) : 0;
     {
         // the shared-memory and cluster-size opt-ins are per-device function attributes
         static std::mutex mu;
@@ -521,7 +524,7 @@ int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
         std::lock_guard<std::mutex> lock(mu);
         if (!ready[dev]) {
             e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)logits_smem(LG_COUNT_BYTES_MAX));
+                                     (int)logits_smem(LG_COUNT_BYTES_MAX, LG_COUNT_BYTES_MAX / 16));
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return fail_cuda(e, "tqk_process_logits: kernel attributes");
@@ -595,19 +598,27 @@ extern "C" int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream)
     p.mask_rows = a->mask_rows;
     p.n_mask_rows = a->n_mask_rows;
     p.err = device_info()->err_word;
-    // CTAs per row: 8, each with at least 2048 tokens, or 16 while all of them run at once (a GPC does not fill up with
-    // clusters of 16, so 3 per SM).  128256 tokens, histories of up to 4000, everything on, 16 against 8 CTAs per row:
-    // 1 row 10.9 and 13.7 us, 24 rows 15.6 and 15.8 us, 37 rows 24.9 and 21.0 us, 256 rows 126 and 86 us (4: 103 us)
-    const int most = (long long)a->n_rows * LG_CLUSTER <= 3LL * device_info()->sm_count ? LG_CLUSTER : 8;
-    while (1 << p.log_c < most && a->vocab_size > 2048 << p.log_c) p.log_c++;
+    // CTAs per row: as few (up to 8) as hold 16384 tokens each, since every one of them scans the row's history, and more
+    // while two of all CTAs per SM suffice and each keeps 2048 tokens.  Everything on, histories of up to 2000:
+    //   30001 tokens, 1, 2, 4 and 8 CTAs per row: 10 rows 20.3, 14.6, 11.3, 10.5 us, 74 rows 24.0, 17.0, 18.4, 21.5 us,
+    //   148 rows 27.3, 22.1, 24.9, 35.8 us, 512 rows 73, 53, 65, 109 us;
+    //   128256 tokens, 8 and 16 (histories of up to 4000): 1 row 13.7, 10.9 us, 24 rows 15.8, 15.6 us, 37 rows 21.0, 24.9 us
+    const long long slots = 2LL * device_info()->sm_count;
+    while (1 << p.log_c < LG_CLUSTER && a->vocab_size > 4096 << p.log_c &&
+           ((1 << p.log_c < LG_CLUSTER / 2 && a->vocab_size > LG_OWN << p.log_c) || (long long)a->n_rows << (p.log_c + 1) <= slots))
+        p.log_c++;
     const int cluster = 1 << p.log_c;
     p.own_blocks = (int)(((int64_t)a->vocab_size + (int64_t)cluster * LG_BLOCK - 1) / ((int64_t)cluster * LG_BLOCK));
     const bool vec = ((reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.out)) & 15) == 0 &&
                      (a->n_rows == 1 || ((ls | (p.out ? os : 0)) & 3) == 0);
     const bool count = penal || a->bias_tokens;
-    // 16 bits per token of the CTA (a long history's 32 bits take two rounds), whole chunks of 32-bit counters
-    const int64_t chunk_bytes = LG_CHUNK * 4, bytes = ((int64_t)p.own_blocks * LG_BLOCK * 2 + chunk_bytes - 1) / chunk_bytes * chunk_bytes;
+    // 32 bits per token of the CTA where one chunk holds them all, else 16 and at least a chunk of 32 (a long history's
+    // counters take more rounds)
+    const int64_t own = (int64_t)p.own_blocks * LG_BLOCK, bytes = own <= LG_CHUNK ? own * 4 : own * 2;
     p.count_bytes = (int)(bytes < LG_COUNT_BYTES_MAX ? bytes : LG_COUNT_BYTES_MAX);
+    if (own > LG_CHUNK && p.count_bytes < LG_CHUNK * 4) p.count_bytes = LG_CHUNK * 4;
+    const int64_t covered = own < LG_COUNT_BYTES_MAX / 2 ? own : LG_COUNT_BYTES_MAX / 2;
+    p.bitmap_bytes = (int)((covered + LG_CHUNK - 1) / LG_CHUNK * (LG_CHUNK / 8));
     cudaStream_t st = (cudaStream_t)stream;
     if (vec) return count ? launch_logits<true, true>(p, cluster, st) : launch_logits<true, false>(p, cluster, st);
     return count ? launch_logits<false, true>(p, cluster, st) : launch_logits<false, false>(p, cluster, st);

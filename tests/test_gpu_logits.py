@@ -108,6 +108,21 @@ def test_against_the_definition(tqk, cuda, rows, vocab, history, biases, share, 
     assert tqk.device_status() == 0
 
 
+MANY_ROWS = [  # few CTAs per row
+    (160, 20001, (0, 12000), (0, 11), 0.5, (1, 1, 1), 0),   # 2, in one or two rounds by the history
+    (600, 1001, (0, 300), (0, 5), 0.9, (1, 1, 1), 3),       # 1 with a part of a chunk
+    (300, 8193, (0, 9000), None, 0.5, (1, 1, 0), 0),        # 1 with a block more than a chunk
+    (76, 140001, (0, 9500), (0, 30), 0.5, (1, 1, 1), 0),    # 8 with more than 16384 tokens each
+    (75, 140004, (0, 9500), (0, 30), 0.5, (0, 1, 1), 0),
+]
+
+
+@pytest.mark.parametrize("mode", ["out", "in place", "choice"])
+@pytest.mark.parametrize("rows,vocab,history,biases,share,penal,pad", MANY_ROWS)
+def test_many_rows(tqk, cuda, rows, vocab, history, biases, share, penal, pad, mode):
+    test_against_the_definition(tqk, cuda, rows, vocab, history, biases, share, penal, pad, mode)
+
+
 def test_ties_go_to_the_lowest_token(tqk, cuda):
     import torch
     for vocab in (100, 40000, 140001):
