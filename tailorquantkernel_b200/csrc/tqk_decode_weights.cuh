@@ -19,11 +19,6 @@ __global__ void __launch_bounds__(WP_THREADS) weight_sum_kernel(const DecodePara
     const int item = blockIdx.z, kvh = blockIdx.y;
     const int t0 = blockIdx.x * (WP_THREADS * WP_TOKENS) + threadIdx.x;
     const long long at = (long long)item * p.stat_stride + (long long)kvh * p.max_tokens;
-    // the sums are loaded before the wait: the decode launched just before this does not write them, and it has itself
-    // waited for every earlier kernel of the stream (an earlier weight pass among them) before letting this one start
-    float old[WP_TOKENS];
-#pragma unroll
-    for (int k = 0; k < WP_TOKENS; k++) old[k] = p.weight[at + min(t0 + k * WP_THREADS, p.len_cap - 1)];
     grid_dependency_wait();
     grid_dependents_launch();
     int len = p.lens ? p.lens[item] : p.len0 + item * p.len_step;
@@ -35,6 +30,10 @@ __global__ void __launch_bounds__(WP_THREADS) weight_sum_kernel(const DecodePara
     int from[WP_TOKENS];  // tokens behind the end load the last one's scores
 #pragma unroll
     for (int k = 0; k < WP_TOKENS; k++) from[k] = min(t0 + k * WP_THREADS, len - 1);
+    // the sums, usually written by the pass before, are in flight together with the first scores
+    float old[WP_TOKENS];
+#pragma unroll
+    for (int k = 0; k < WP_TOKENS; k++) old[k] = p.weight[at + from[k]];
     float w[WP_TOKENS] = {};
     for (int g0 = 0; g0 < p.group; g0 += WP_HEADS) {
         float s[WP_HEADS][WP_TOKENS];
