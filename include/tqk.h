@@ -218,6 +218,8 @@ TQK_API int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t work
  * Results do not depend on the run: sums are added in a fixed order.
  *   - Lengths read from the device are clamped to max_len here (the workspace
  *     holds no more scores), reported as TQK_EDEVLEN.
+ *   - Where a bounded wait gives up (TQK_ETIMEOUT), the heads whose softmax was not
+ *     finished keep their sums and positions; the others have theirs added.
  *   - The workspace holds the decode's tickets and partials and one float per
  *     q head and position: tqk_decode_weights_workspace_size() bytes, under
  *     tqk_decode_q8's rules (zeroed once, ordered on one stream, shared with

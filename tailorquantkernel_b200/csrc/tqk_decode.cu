@@ -116,6 +116,13 @@ enum : int { WT_NONE = 0, WT_NAT = 1, WT_LOG2 = 2 };
 __device__ __forceinline__ float *score_row_of(const DecodeParams &p, int item, int qh) {
     return p.scores + ((long long)item * (p.n_kv * p.group) + qh) * p.score_stride;
 }
+// Whether a q head's softmax is whole: its (max, sum) entry starts every call as "not yet", from the CTA of its unit's first
+// split, and only the merge of all splits replaces that.  The weight pass leaves the sums of a unit alone whose decode
+// gave up on a wait; without this it would add what the workspace holds of an earlier call.
+__device__ __forceinline__ void set_unfinished(const DecodeParams &p, int item, int qh) {
+    p.ml[(long long)item * (p.n_kv * p.group) + qh] = make_float2(0.0f, -1.0f);
+}
+__device__ __forceinline__ bool is_unfinished(float2 ml) { return ml.y < 0.0f; }  // no sum of exponentials is negative
 // A bulk copy of the K / V stream.  With scores to keep, the rows (read once per call) are the first to leave L2, so
 // that the scores are still there for the weight pass.
 template <int WT>
@@ -504,6 +511,7 @@ __global__ void __launch_bounds__(DEC_THREADS) decode_q8_kernel(const DecodePara
         return;
     }
 
+    if (WT != WT_NONE && s == 0 && tid < G) set_unfinished(p, item, qh0 + tid);
     const int t_begin = s * p.split_tokens;
     const int t_end = split_end(s, n_splits, p.split_tokens, len);
     const int n_tiles = (t_end - t_begin + DEC_T - 1) / DEC_T;

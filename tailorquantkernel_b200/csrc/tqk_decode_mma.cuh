@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(MMA_THREADS) decode_q8_mma_kernel(const Decode
         return;
     }
 
+    if (WT != WT_NONE && s == 0 && tid < G) set_unfinished(p, item, qh0 + tid);
     const int t_begin = s * p.split_tokens;
     const int t_end = split_end(s, n_splits, p.split_tokens, len);
     const int n_tiles = (t_end - t_begin + MMA_T - 1) / MMA_T;

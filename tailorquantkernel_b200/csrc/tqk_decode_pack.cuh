@@ -460,12 +460,12 @@ __device__ __forceinline__ void pack_reduce(const PackState<NB> &st, const PackR
 // rank order -- and writes them; then it arrives on every other CTA's cbar[1]
 // and leaves only when its own cbar[1] completes, i.e. when no CTA reads its
 // shared memory any more.  Every wait is bounded (the error word records a
-// timeout).  empty: this CTA holds no keys, or gave up on a wait.  Run by the
-// consumer threads only.
+// timeout).  empty: this CTA holds no keys, or gave up on a wait (gave_up: a
+// sum of -1 tells the others so).  Run by the consumer threads only.
 constexpr uint64_t CL_WAIT_NS = 2000000000ull;  // above the 1 s bound of every wait before the merge
 template <int NB, int WT>
 __device__ __forceinline__ void pack_cluster_merge(const DecodeParams &p, uint8_t *smem, const PackRed &r, bool empty,
-                                                   int tid, int item, int qh0, float *out_item) {
+                                                   bool gave_up, int tid, int item, int qh0, float *out_item) {
     using L = PackLayout<NB>;
     constexpr int HD = L::HD, NT = PK_WARPS * 32, E = 8 * HD;
     constexpr int KV = (E + CL_MAX + NT - 1) / NT;  // (element, rank) values per thread
@@ -481,7 +481,7 @@ __device__ __forceinline__ void pack_cluster_merge(const DecodeParams &p, uint8_
     for (int i = tid; i < E; i += NT) cp[i] = empty ? 0.0f : r.acc<L::RED_STRIDE>(i / HD, i % HD);
     if (tid < 8) {
         cp[E + tid] = empty ? -INFINITY : r.fm()[tid];
-        cp[E + 8 + tid] = empty ? 0.0f : r.fl()[tid];
+        cp[E + 8 + tid] = gave_up ? -1.0f : empty ? 0.0f : r.fl()[tid];
     }
     if (tid == 0) *okf = 1;
     cta_sync<1, NT>();  // the partial is complete (and the reduction rows are free)
@@ -515,15 +515,17 @@ __device__ __forceinline__ void pack_cluster_merge(const DecodeParams &p, uint8_
             float M = -INFINITY;
             for (int rr = 0; rr < C; rr++) M = fmaxf(M, cm[rr * 8 + tid]);
             float Ls = 0.0f;
+            bool whole = true;
             for (int rr = 0; rr < C; rr++) {
                 const float m = cm[rr * 8 + tid];
                 const float w = m == -INFINITY ? 0.0f : WT == WT_LOG2 ? exp2f(m - M) : expf(m - M);
                 cm[rr * 8 + tid] = w;
                 Ls += cl[rr * 8 + tid] * w;
+                if (WT != WT_NONE) whole &= !(cl[rr * 8 + tid] < 0.0f);
             }
             fin[tid] = M;
             fin[8 + tid] = Ls;
-            if (WT != WT_NONE && rank == 0)
+            if (WT != WT_NONE && rank == 0 && whole)
                 p.ml[(long long)item * (p.n_kv * p.group) + qh0 + tid] = make_float2(M, Ls);
         }
         cta_sync<1, NT>();
@@ -593,7 +595,8 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
         // partial); with len == 0 every CTA of the cluster (one item) leaves here or just below
         if (clustered && len > 0 && warp < PK_WARPS) {
             float *red = reinterpret_cast<float *>(smem);
-            pack_cluster_merge<NB, WT>(p, smem, PackRed{red, red + L::RED_FLOATS}, true, tid, item, qh0, out_item);
+            pack_cluster_merge<NB, WT>(p, smem, PackRed{red, red + L::RED_FLOATS}, true, false, tid, item, qh0,
+                                       out_item);
         }
         return;
     }
@@ -612,6 +615,7 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
         return;
     }
 
+    if (WT != WT_NONE && s == 0 && tid < G) set_unfinished(p, item, qh0 + tid);
     const int t_begin = s * p.split_tokens;
     const int t_end = split_end(s, n_splits, p.split_tokens, len);
     const int n_tiles = (t_end - t_begin + PK_T - 1) / PK_T;
@@ -715,13 +719,13 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_kernel
     float *red = reinterpret_cast<float *>(smem);  // [W][8][RED_STRIDE]
     PackRed r{red, red + L::RED_FLOATS};
     if (*timeout) {
-        if (clustered) pack_cluster_merge<NB, WT>(p, smem, r, true, tid, item, qh0, out_item);
+        if (clustered) pack_cluster_merge<NB, WT>(p, smem, r, true, true, tid, item, qh0, out_item);
         return;
     }
 
     pack_reduce<NB, L::RED_STRIDE, WT>(st, r, warp, g, t, tid);
     if (clustered) {
-        pack_cluster_merge<NB, WT>(p, smem, r, false, tid, item, qh0, out_item);
+        pack_cluster_merge<NB, WT>(p, smem, r, false, false, tid, item, qh0, out_item);
         return;
     }
     float *wts = r.fl() + 8;                       // [2][MAX_SPLITS][8]
@@ -936,6 +940,14 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
         const int Tn = pre[n_items], Cn = min((int)gridDim.x, Tn);
         return (int)((long long)(blockIdx.x + 1) * Tn / Cn);
     };
+    if (WT != WT_NONE && warp == 0) {
+        // ahead of every wait: a CTA that gives up reaches none of its later units
+        for (int gt = g0; gt < g1;) {
+            const BalSeg sg = bal_segment(pre, lens, n_items, pairs, gt, g1);
+            if (sg.lt0 == 0 && lane < G) set_unfinished(p, sg.item, 2 * sg.pair * p.group + lane);
+            gt = sg.ubase + sg.lt1;
+        }
+    }
     int j = 0;  // ring position of the next tile
     for (int gt = g0;;) {
         {

@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(WP_THREADS) weight_sum_kernel(const DecodePara
 #pragma unroll
     for (int k = 0; k < WP_TOKENS; k++) old[k] = p.weight[at + from[k]];
     float w[WP_TOKENS] = {};
+    bool whole = true;
     for (int g0 = 0; g0 < p.group; g0 += WP_HEADS) {
         float s[WP_HEADS][WP_TOKENS];
         float2 ml[WP_HEADS];
@@ -48,6 +49,7 @@ __global__ void __launch_bounds__(WP_THREADS) weight_sum_kernel(const DecodePara
 #pragma unroll
         for (int g = 0; g < WP_HEADS; g++) {
             if (g0 + g >= p.group) break;
+            whole &= !is_unfinished(ml[g]);
             const float inv = __fdiv_rn(1.0f, ml[g].y);
 #pragma unroll
             for (int k = 0; k < WP_TOKENS; k++) {
@@ -56,6 +58,7 @@ __global__ void __launch_bounds__(WP_THREADS) weight_sum_kernel(const DecodePara
             }
         }
     }
+    if (!whole) return;  // the decode gave up on a wait (and recorded it)
 #pragma unroll
     for (int k = 0; k < WP_TOKENS; k++) {
         const int t = t0 + k * WP_THREADS;

@@ -44,3 +44,38 @@ def test_calls_back_to_back_add_to_each_other(tqk, cuda, nq, nkv, hd, mt, lens, 
     for i, n in enumerate(lens):  # every call added weights that sum to the group's q heads; each addition rounds once
         added = (got[i, :, :n].astype(np.float64) - c.weight[i, :, :n]).sum(-1)
         assert np.abs(added - 50 * nq / nkv).max() < 50 * nq / nkv * 1e-5 + 50 * n * 2.0 ** -24 * got[i, :, :n].max()
+
+
+@pytest.mark.parametrize("nq,nkv,hd,mt,lens,split,unit_heads", [
+    (8, 4, 128, 300, [300, 300], 64, 1),           # unpacked tensor-core kernel
+    (16, 4, 128, 300, [300, 200], 64, 2),          # packed: a unit is two kv heads
+    (40, 2, 128, 300, [300, 300], 64, 1),          # two units per kv head: one of them is enough
+    (4, 2, 64, 300, [300, 150], 64, 1),            # CUDA cores
+    (8, 2, 128, 9000, [9000], -1, 2),              # balanced schedule, one unit over many CTAs
+])
+def test_a_decode_that_gives_up_adds_nothing(tqk, cuda, nq, nkv, hd, mt, lens, split, unit_heads):
+    """A unit whose splits are never merged -- what a wait that runs out leaves behind, made here by a merge ticket that no
+    split can complete -- keeps its sums and positions; the other units get theirs."""
+    import torch
+    c = Case(tqk, 81 + hd, nq, nkv, hd, mt, lens, device_lens=True)
+    a, w = c.args(split), c.wargs()
+    ws = torch.zeros(tqk.decode_weights_workspace_size(a) // 4 * 4, dtype=torch.uint8, device="cuda")
+    before = c.dw.clone()
+    tqk.decode_weights(a, c.wargs(c.dw.clone()), ws)   # leaves plausible scores, maxima and sums in the workspace
+    c.dpos.fill_(-5)
+    c.dq.copy_(torch.randn(c.dq.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+    want = c.dw.clone()
+    tqk.decode_weights(a, c.wargs(want), ws)
+    c.dpos.fill_(-5)
+    # the first ticket of the last item's last unit; 17 tickets a unit
+    units = nkv // unit_heads * -(-(nq // nkv) // 16)  # 16 q heads at most in a unit of the unpacked kernels
+    ws.view(torch.int32)[17 * (len(lens) * units - 1)] = 1000
+    tqk.decode_weights(a, w, ws)
+    torch.cuda.synchronize()
+    got, kept, full = (c.item(t, nkv * mt).reshape(len(lens), nkv, mt).view(np.int32) for t in (c.dw, before, want))
+    heads = slice(nkv - unit_heads, nkv)
+    full[-1, heads] = kept[-1, heads]
+    assert np.array_equal(got, full)
+    pos = c.item(c.dpos, nkv * mt).reshape(len(lens), nkv, mt)
+    assert (pos[-1, heads] == -5).all()
+    assert len(lens) == 1 or pos[0, 0, lens[0] - 1] == 1000
