@@ -200,8 +200,10 @@ TQK_API int tqk_decode_workspace_size(const tqk_decode_args *a, size_t *bytes);
  * units) can reuse it without re-initialising.  Zero it again before a call
  * with more units than any earlier one, and after a call that reported
  * TQK_ETIMEOUT.  Calls that share a workspace must be ordered on one stream.
- * workspace == NULL uses a library-owned workspace per (device, stream),
- * allocated on first use, whose tickets live apart from the partials. */
+ * workspace == NULL uses a library-owned workspace per (device, stream; for
+ * cudaStreamPerThread, whose handle is a stream of its own in every host thread,
+ * also per thread), allocated on first use and kept, whose tickets live apart from
+ * the partials. */
 TQK_API int tqk_workspace_init(void *workspace, size_t bytes, tqk_stream_t stream);
 TQK_API int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t workspace_bytes, tqk_stream_t stream);
 

@@ -1,12 +1,12 @@
 // tqk_runtime.cu -- status codes, per-thread error text, per-device state and
 // the library-owned workspaces behind the tqk C ABI.
 #include "tqk_internal.h"
+#include "tqk_stream_key.h"
 
 #include <cstdio>
 #include <cstring>
 #include <map>
 #include <mutex>
-#include <utility>
 
 namespace tqk {
 
@@ -20,10 +20,10 @@ struct Workspace {
     void *ptr = nullptr;
     size_t bytes = 0;
 };
-std::map<std::pair<int, cudaStream_t>, Workspace> g_workspaces;
-std::map<std::pair<int, cudaStream_t>, Workspace> g_counters;
-std::map<std::pair<int, cudaStream_t>, Workspace> g_scratch;
-std::map<std::pair<int, cudaStream_t>, Workspace> g_prefill_stage;
+std::map<StreamKey, Workspace> g_workspaces;
+std::map<StreamKey, Workspace> g_counters;
+std::map<StreamKey, Workspace> g_scratch;
+std::map<StreamKey, Workspace> g_prefill_stage;
 
 // Grows `w` to at least `bytes` (minimum 1 MiB), zeroing the new buffer on `stream`.
 void *grow_zeroed(Workspace &w, cudaStream_t stream, size_t bytes) {
@@ -95,28 +95,28 @@ void *library_workspace(cudaStream_t stream, size_t bytes) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
     std::lock_guard<std::mutex> lock(g_mutex);
-    return grow_zeroed(g_workspaces[{dev, stream}], stream, bytes);
+    return grow_zeroed(g_workspaces[stream_key(dev, stream)], stream, bytes);
 }
 
 int *library_counters(cudaStream_t stream, size_t bytes) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
     std::lock_guard<std::mutex> lock(g_mutex);
-    return static_cast<int *>(grow_zeroed(g_counters[{dev, stream}], stream, bytes));
+    return static_cast<int *>(grow_zeroed(g_counters[stream_key(dev, stream)], stream, bytes));
 }
 
 void *library_scratch(cudaStream_t stream, size_t bytes) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
     std::lock_guard<std::mutex> lock(g_mutex);
-    return grow_zeroed(g_scratch[{dev, stream}], stream, bytes);
+    return grow_zeroed(g_scratch[stream_key(dev, stream)], stream, bytes);
 }
 
 void *library_prefill_stage(cudaStream_t stream, size_t bytes) {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
     std::lock_guard<std::mutex> lock(g_mutex);
-    return grow_zeroed(g_prefill_stage[{dev, stream}], stream, bytes);
+    return grow_zeroed(g_prefill_stage[stream_key(dev, stream)], stream, bytes);
 }
 
 }  // namespace tqk

@@ -186,3 +186,29 @@ def test_plain_attention_sums_to_one_per_head():
     q, k, v = (port.quantize_rows(rng.standard_normal(s, dtype=np.float32)) for s in ((2, 6, 64), (2, 2, 9, 64), (2, 2, 9, 64)))
     _, w, big = attend64(q, k, v, [9, 4])
     assert np.allclose(w.sum(-1), 3.0) and (w[1, :, 4:] == 0).all() and 0 < weight_bound(2, big, 9) < 1e-5
+
+
+def test_library_buffers_of_the_per_thread_stream_belong_to_a_thread(tmp_path):
+    """The key of the library-owned workspaces: one handle, cudaStreamPerThread, is another stream in every thread."""
+    from tailorquantkernel_b200 import build
+    src, exe = tmp_path / "key.cpp", tmp_path / "key"
+    src.write_text('#include <cstdio>\n#include <set>\n#include <thread>\n#include <vector>\n#include "tqk_stream_key.h"\n'
+                   "using namespace tqk;\n"
+                   "int main() {\n"
+                   "  cudaStream_t own = reinterpret_cast<cudaStream_t>(64);\n"
+                   "  std::vector<StreamKey> got(16, StreamKey{});\n"
+                   "  // one thread after the other, so that their ids may be the same\n"
+                   "  for (int i = 0; i < 8; i++) std::thread([&, i] {\n"
+                   "    got[2 * i] = stream_key(i % 2, cudaStreamPerThread);\n"
+                   "    got[2 * i + 1] = stream_key(i % 2, own);\n"
+                   "    StreamKey again = stream_key(i % 2, cudaStreamPerThread);\n"
+                   "    if (again < got[2 * i] || got[2 * i] < again) got[2 * i + 1].thread = 99;\n"
+                   "  }).join();\n"
+                   "  std::set<StreamKey> keys(got.begin(), got.end());\n"
+                   '  std::printf("%zu", keys.size());\n'
+                   "}\n")
+    cuda = os.path.dirname(os.path.dirname(build._nvcc()))
+    subprocess.run(["/usr/bin/g++", "-std=c++17", "-pthread", "-I", build.CSRC, "-I", os.path.join(cuda, "include"), str(src),
+                    "-o", str(exe)], check=True)
+    # 8 threads' own streams, and one other stream on each of two devices
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "10"

@@ -79,3 +79,43 @@ def test_a_decode_that_gives_up_adds_nothing(tqk, cuda, nq, nkv, hd, mt, lens, s
     pos = c.item(c.dpos, nkv * mt).reshape(len(lens), nkv, mt)
     assert (pos[-1, heads] == -5).all()
     assert len(lens) == 1 or pos[0, 0, lens[0] - 1] == 1000
+
+
+def test_two_threads_on_their_per_thread_streams(tqk, cuda):
+    """cudaStreamPerThread is one handle and a stream per thread: each thread has library buffers of its own, also while the
+    other's grow."""
+    import threading
+    import torch
+    lens = [[40], [2000], [300], [4000], [70], [900]]
+    cases = [[Case(tqk, 91 + 10 * t + i, 8, 2, 128, n[0], n, append=False) for i, n in enumerate(lens)] for t in range(2)]
+    want = []
+    for cs in cases:
+        for c in cs:
+            dw = c.dw.clone()
+            tqk.decode_weights(c.args(64), c.wargs(dw))
+            want.append((c.out.clone(), dw))
+            c.out.fill_(float("nan"))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(cs):
+        try:
+            for _ in range(20):
+                for c in cs:
+                    tqk.decode_weights(c.args(64), c.wargs(c.after), stream=2)
+        except Exception as e:  # seen by the test
+            failed.append(e)
+
+    for cs in cases:
+        for c in cs:
+            c.after = torch.full_like(c.dw, float("nan"))
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(cs,)) for cs in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for c, (out, dw) in zip(cases[0] + cases[1], want):
+        assert torch.equal(c.out, out) and torch.equal(_bits(c.after), _bits(dw))
