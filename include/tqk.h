@@ -203,7 +203,9 @@ TQK_API int tqk_decode_workspace_size(const tqk_decode_args *a, size_t *bytes);
  * workspace == NULL uses a library-owned workspace per (device, stream; for
  * cudaStreamPerThread, whose handle is a stream of its own in every host thread,
  * also per thread), allocated on first use and kept, whose tickets live apart from
- * the partials. */
+ * the partials.  A captured call needs one that is large enough from an earlier
+ * call outside capture (TQK_ECUDA otherwise), and its graph keeps it: larger calls
+ * that follow get another. */
 TQK_API int tqk_workspace_init(void *workspace, size_t bytes, tqk_stream_t stream);
 TQK_API int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t workspace_bytes, tqk_stream_t stream);
 

@@ -19,21 +19,30 @@ DeviceInfo g_devices[64];
 struct Workspace {
     void *ptr = nullptr;
     size_t bytes = 0;
+    bool captured = false;  // a captured call holds this buffer: its graph may be replayed whenever the caller likes
 };
 std::map<StreamKey, Workspace> g_workspaces;
 std::map<StreamKey, Workspace> g_counters;
 std::map<StreamKey, Workspace> g_scratch;
 std::map<StreamKey, Workspace> g_prefill_stage;
 
-// Grows `w` to at least `bytes` (minimum 1 MiB), zeroing the new buffer on `stream`.
+// Grows `w` to at least `bytes` (minimum 1 MiB), zeroing the new buffer on `stream`.  A buffer that a graph was captured
+// with is left to that graph for good when a larger one is needed; nothing grows while `stream` is captured.
 void *grow_zeroed(Workspace &w, cudaStream_t stream, size_t bytes) {
-    if (w.bytes >= bytes && w.ptr) return w.ptr;
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess) (void)cudaGetLastError();
+    if (w.bytes >= bytes && w.ptr) {
+        if (capturing != cudaStreamCaptureStatusNone) w.captured = true;
+        return w.ptr;
+    }
     if (w.ptr) {
-        // the old buffer may still be in use by work queued on `stream`
-        cudaStreamSynchronize(stream);
-        cudaFree(w.ptr);
-        w.ptr = nullptr;
-        w.bytes = 0;
+        if (capturing != cudaStreamCaptureStatusNone) return nullptr;
+        if (!w.captured) {
+            // the old buffer may still be in use by work queued on `stream`
+            cudaStreamSynchronize(stream);
+            cudaFree(w.ptr);
+        }
+        w = Workspace{};
     }
     size_t grow = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
     if (cudaMalloc(&w.ptr, grow) != cudaSuccess) {
@@ -43,6 +52,7 @@ void *grow_zeroed(Workspace &w, cudaStream_t stream, size_t bytes) {
     }
     if (cudaMemsetAsync(w.ptr, 0, grow, stream) != cudaSuccess) return nullptr;
     w.bytes = grow;
+    w.captured = capturing != cudaStreamCaptureStatusNone;
     return w.ptr;
 }
 }  // namespace

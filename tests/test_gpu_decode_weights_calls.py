@@ -119,3 +119,32 @@ def test_two_threads_on_their_per_thread_streams(tqk, cuda):
     assert not failed
     for c, (out, dw) in zip(cases[0] + cases[1], want):
         assert torch.equal(c.out, out) and torch.equal(_bits(c.after), _bits(dw))
+
+
+def test_a_captured_decode_keeps_its_library_workspace(tqk, cuda):
+    """A graph of tqk_decode_q8 with the library's workspace, replayed after larger calls on its stream made that grow."""
+    import torch
+    small, large = Case(tqk, 101, 8, 2, 128, 700, [700]), Case(tqk, 102, 32, 8, 128, 3000, [3000] * 8, append=False)
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    tqk.decode(small.args(64), stream=s)
+    s.synchronize()
+    want = small.out.clone()
+    small.out.fill_(float("nan"))
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        tqk.decode(small.args(64))
+        with pytest.raises(tqk.TQKError):  # no growth under capture, which goes on
+            tqk.decode(large.args(64))
+    tqk.decode_weights(large.args(64), large.wargs(), stream=s)   # grows
+    s.synchronize()
+    junk = [torch.full((1 << 18,), float("nan"), device="cuda") for _ in range(64)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(s):
+            g.replay()
+        tqk.decode_weights(large.args(64), large.wargs(), stream=s)
+        s.synchronize()
+        assert torch.equal(small.out, want)
+        small.out.fill_(float("nan"))
+        torch.cuda.synchronize()
+    assert all(t.isnan().all() for t in junk)
