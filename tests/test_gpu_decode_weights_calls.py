@@ -148,3 +148,24 @@ def test_a_captured_decode_keeps_its_library_workspace(tqk, cuda):
         small.out.fill_(float("nan"))
         torch.cuda.synchronize()
     assert all(t.isnan().all() for t in junk)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,mt,lens,device_lens", [
+    (8, 1, 128, 64, [64], False), (7, 1, 128, 65, [65, 64, 1], True),         # 8 rows; the limit and one above it
+    (16, 1, 128, 40, [40], False), (15, 1, 128, 66, [64, 33, 0, 17], True),   # 16 rows
+    (16, 1, 256, 33, [33], False), (6, 2, 256, 64, [64, 63], False),          # head_dim 256, 16 and 8 rows
+    (12, 3, 128, 64, [17, 16, 15], False), (2, 2, 128, 64, [1, 2], False),
+    (32, 2, 128, 50, [50, 49], False), (34, 2, 128, 50, [50, 49], False),     # one slice of 16; two slices: not fused
+    (16, 4, 128, 64, [64, 64], False), (16, 4, 128, 65, [65, 65], False),     # packed
+])
+@pytest.mark.parametrize("append", [True, False])
+def test_short_caches_add_their_weights_in_the_decode(tqk, cuda, nq, nkv, hd, mt, lens, device_lens, append):
+    """Every tensor-core kernel on both sides of the length up to which it adds the weights itself."""
+    import torch
+    c = Case(tqk, nq * 100 + mt, nq, nkv, hd, mt, lens, append, device_lens, pad=3)
+    after = c.dw.clone()
+    tqk.decode_weights(c.args(), c.wargs(after))
+    torch.cuda.synchronize()
+    c.check(after)
+    tqk.decode_weights(c.args(), c.wargs())
+    assert torch.equal(_bits(c.dw), _bits(after)) and tqk.device_status() == 0
