@@ -21,6 +21,7 @@
 //   * each CTA pushes its candidate for the greedy choice to the first CTA's
 //     shared memory; a cluster barrier later the first CTA compares them.
 #include "tqk_internal.h"
+#include "tqk_logits_plan.h"
 
 #include <climits>
 #include <mutex>
@@ -34,8 +35,6 @@ constexpr int LG_WARPS = LG_THREADS / 32;
 constexpr int LG_BLOCK = 128;                            // tokens per block: a warp's 16-byte loads
 constexpr int LG_LOADS = 8;                              // blocks per warp and chunk, in registers
 constexpr int LG_CHUNK = LG_WARPS * LG_LOADS * LG_BLOCK; // 8192 tokens
-constexpr int LG_CLUSTER = 16;                           // most CTAs per row (non-portable above 8), a power of two
-constexpr int LG_OWN = 16384;                            // tokens per CTA, from which more CTAs take a row
 constexpr int LG_COUNT_BYTES_MAX = 64 << 10;             // counters per CTA
 constexpr int LG_LIST = 256;                             // listed tokens per warp at a time
 constexpr int LG_SCAN = 4 * LG_THREADS;                  // history entries staged at a time: a 16-byte copy per thread
@@ -511,26 +510,47 @@ __global__ void __launch_bounds__(LG_THREADS, 4) logits_kernel(const LogitsParam
 // 4 CTAs of 51 KB only 28 KB (256 rows of 128256 tokens: 111 and 121 us).
 size_t logits_smem(int count_bytes, int bitmap_bytes) { return count_bytes + bitmap_bytes + LG_STAGE * 4 + LG_WARPS * LG_LIST * 2; }
 
+// Sets up the kernel on the current device, once: the shared-memory and cluster-size opt-ins are per-device function
+// attributes.  *most: CTAs per row, 16 where the device holds such a cluster (a part of a device may not), else 8.
+template <bool VEC, bool COUNT>
+int prepare_logits(int *most) {
+    constexpr auto kernel = logits_kernel<VEC, COUNT>;
+    static std::mutex mu;
+    static int most_by[64];  // 0 = not set up
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64) return fail_cuda(e, "tqk_process_logits: cudaGetDevice");
+    std::lock_guard<std::mutex> lock(mu);
+    if (!most_by[dev]) {
+        const int smem = (int)logits_smem(LG_COUNT_BYTES_MAX, LG_COUNT_BYTES_MAX / 16);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return fail_cuda(e, "tqk_process_logits: kernel attributes");
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        int n = 0;
+        if (e == cudaSuccess) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(LG_CLUSTER, 1, 1);
+            cfg.blockDim = dim3(LG_THREADS);
+            cfg.dynamicSmemBytes = COUNT ? smem : 0;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = LG_CLUSTER;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+        }
+        if (e != cudaSuccess) (void)cudaGetLastError();  // not an error of the call: smaller clusters
+        most_by[dev] = e == cudaSuccess && n > 0 ? LG_CLUSTER : LG_CLUSTER_PORTABLE;
+    }
+    *most = most_by[dev];
+    return TQK_OK;
+}
+
 template <bool VEC, bool COUNT>
 int launch_logits(const LogitsParams &p, int cluster, cudaStream_t stream) {
     const size_t smem = COUNT ? logits_smem(p.count_bytes, p.bitmap_bytes) : 0;
-    {
-        // the shared-memory and cluster-size opt-ins are per-device function attributes
-        static std::mutex mu;
-        static bool ready[64];
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess || dev < 0 || dev >= 64) return fail_cuda(e, "tqk_process_logits: cudaGetDevice");
-        std::lock_guard<std::mutex> lock(mu);
-        if (!ready[dev]) {
-            e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)logits_smem(LG_COUNT_BYTES_MAX, LG_COUNT_BYTES_MAX / 16));
-            if (e == cudaSuccess)
-                e = cudaFuncSetAttribute(logits_kernel<VEC, COUNT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-            if (e != cudaSuccess) return fail_cuda(e, "tqk_process_logits: kernel attributes");
-            ready[dev] = true;
-        }
-    }
     const dim3 grid((unsigned)cluster, (unsigned)p.n_rows);
     if (cluster == 1) return launch_pdl(logits_kernel<VEC, COUNT>, grid, dim3(LG_THREADS), smem, stream, p);
     return launch_pdl_cluster(logits_kernel<VEC, COUNT>, grid, dim3(LG_THREADS), smem, stream, (unsigned)cluster, p);
@@ -598,20 +618,16 @@ extern "C" int tqk_process_logits(const tqk_logits_args *a, tqk_stream_t stream)
     p.mask_rows = a->mask_rows;
     p.n_mask_rows = a->n_mask_rows;
     p.err = device_info()->err_word;
-    // CTAs per row: as few (up to 8) as hold 16384 tokens each, since every one of them scans the row's history, and more
-    // while two of all CTAs per SM suffice and each keeps 2048 tokens.  Everything on, histories of up to 2000:
-    //   30001 tokens, 1, 2, 4 and 8 CTAs per row: 10 rows 20.3, 14.6, 11.3, 10.5 us, 74 rows 24.0, 17.0, 18.4, 21.5 us,
-    //   148 rows 27.3, 22.1, 24.9, 35.8 us, 512 rows 73, 53, 65, 109 us;
-    //   128256 tokens, 8 and 16 (histories of up to 4000): 1 row 13.7, 10.9 us, 24 rows 15.8, 15.6 us, 37 rows 21.0, 24.9 us
-    const long long slots = 2LL * device_info()->sm_count;
-    while (1 << p.log_c < LG_CLUSTER && a->vocab_size > 4096 << p.log_c &&
-           ((1 << p.log_c < LG_CLUSTER / 2 && a->vocab_size > LG_OWN << p.log_c) || (long long)a->n_rows << (p.log_c + 1) <= slots))
-        p.log_c++;
-    const int cluster = 1 << p.log_c;
-    p.own_blocks = (int)(((int64_t)a->vocab_size + (int64_t)cluster * LG_BLOCK - 1) / ((int64_t)cluster * LG_BLOCK));
     const bool vec = ((reinterpret_cast<uintptr_t>(p.logits) | reinterpret_cast<uintptr_t>(p.out)) & 15) == 0 &&
                      (a->n_rows == 1 || ((ls | (p.out ? os : 0)) & 3) == 0);
     const bool count = penal || a->bias_tokens;
+    int most = 0;
+    rc = vec ? count ? prepare_logits<true, true>(&most) : prepare_logits<true, false>(&most)
+             : count ? prepare_logits<false, true>(&most) : prepare_logits<false, false>(&most);
+    if (rc) return rc;
+    p.log_c = logits_cluster_log(a->n_rows, a->vocab_size, device_info()->sm_count, most);
+    const int cluster = 1 << p.log_c;
+    p.own_blocks = (int)(((int64_t)a->vocab_size + (int64_t)cluster * LG_BLOCK - 1) / ((int64_t)cluster * LG_BLOCK));
     // 32 bits per token of the CTA where one chunk holds them all, else 16 and at least a chunk of 32 (a long history's
     // counters take more rounds)
     const int64_t own = (int64_t)p.own_blocks * LG_BLOCK, bytes = own <= LG_CHUNK ? own * 4 : own * 2;

@@ -212,3 +212,28 @@ def test_library_buffers_of_the_per_thread_stream_belong_to_a_thread(tmp_path):
                     "-o", str(exe)], check=True)
     # 8 threads' own streams, and one other stream on each of two devices
     assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "10"
+
+
+def test_logit_clusters_fit_the_device(tmp_path):
+    """CTAs per row: never more than the device holds in a cluster, and otherwise the measured choices."""
+    from tailorquantkernel_b200 import build
+    src, exe = tmp_path / "plan.cpp", tmp_path / "plan"
+    src.write_text('#include <cstdio>\n#include <cstdlib>\n#include "tqk_logits_plan.h"\n'
+                   "int main(int n, char **v) {\n"
+                   "  for (int i = 1; i + 3 < n; i += 4)\n"
+                   '    std::printf("%d ", 1 << tqk::logits_cluster_log(atoi(v[i]), atoi(v[i + 1]), atoi(v[i + 2]), atoi(v[i + 3])));\n'
+                   "}\n")
+    subprocess.run(["/usr/bin/g++", "-std=c++17", "-I", build.CSRC, str(src), "-o", str(exe)], check=True)
+
+    def ctas(*cases):
+        got = subprocess.run([str(exe)] + [str(x) for c in cases for x in c], capture_output=True, text=True, check=True)
+        return [int(x) for x in got.stdout.split()]
+
+    rows = [1, 2, 7, 18, 19, 37, 74, 148, 256, 512, 65535]
+    vocabs = [1, 4096, 4097, 8192, 8193, 16385, 32003, 65537, 128256, 262144, 2 ** 29 - 1]
+    for sms in (148, 16, 1):
+        cases = [(r, v, sms) for r in rows for v in vocabs]
+        wide, narrow = ctas(*((*c, 16) for c in cases)), ctas(*((*c, 8) for c in cases))
+        assert max(narrow) <= 8 and all(n == min(w, 8) for w, n in zip(wide, narrow))
+    assert ctas((1, 128256, 148, 16), (37, 128256, 148, 16), (256, 128256, 148, 16), (512, 30001, 148, 16),
+                (512, 8001, 148, 16), (10, 30001, 148, 16), (7, 4096, 148, 16)) == [16, 8, 8, 2, 1, 8, 1]
