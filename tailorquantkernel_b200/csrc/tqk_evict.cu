@@ -490,7 +490,7 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
     int rc = ensure_device();
     if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
-    if (max_len > 0) {
+    if (max_len > 0 || a->lens || a->lens_out) {  // also where max_len is 0: device lengths above it are reported
         EvictParams p{};
         p.k = reinterpret_cast<uint8_t *>(a->k);
         p.v = reinterpret_cast<uint8_t *>(a->v);
@@ -542,7 +542,7 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
                        : dispatch_evict<EV_THREADS, false>(nb, p, cluster, grid, st);
         if (rc) return rc;
     }
-    if (!a->lens_out || (max_len > 0 && a->lens_out != a->lens)) return TQK_OK;
+    if (!a->lens_out || a->lens_out != a->lens) return TQK_OK;
     return launch_pdl(evict_lens_kernel, dim3((unsigned)((a->n_items + 255) / 256)), dim3(256), 0, st, a->lens, a->len0,
                       a->len_step, max_len, a->budget, a->n_items, a->lens_out);
 }
