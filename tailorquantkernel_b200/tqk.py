@@ -48,6 +48,8 @@ _sz = ctypes.c_size_t
 
 class DecodeArgs(ctypes.Structure):
     """Mirror of tqk_decode_args (include/tqk.h)."""
+    _keep = ()  # the tensors it was made from, if any
+    _devices = frozenset()  # ... and theirs
     _fields_ = [
         ("k", _vp), ("v", _vp),
         ("item_stride", _i64),
@@ -375,12 +377,13 @@ def decode_args(k, v, n_q, n_kv, head_dim, max_tokens, q, out, *, n_items=1, ite
                 len0=0, len_step=0, max_len=0, q_item_stride=0, out_item_stride=0, k_new=None, v_new=None,
                 kv_new_item_stride=0, out_mode=OUT_NORMALIZED, split_tokens=0, q_norm=None, k_norm=None,
                 norm_item_stride=0, norm_eps=1e-6, rope_cos=None, rope_sin=None, rope_item_stride=0) -> DecodeArgs:
+    """tqk_decode_args.  The struct keeps its tensors alive."""
     a = DecodeArgs()
     a.k, a.v = _ptr(k), _ptr(v)
     a.item_stride = item_stride_blocks
     a.n_items = n_items
     a.n_q_heads, a.n_kv_heads, a.head_dim, a.max_tokens = n_q, n_kv, head_dim, max_tokens
-    a.lens = _ptr(lens)
+    a.lens = _typed(lens, "int32")
     a.len0, a.len_step, a.max_len = len0, len_step, max_len
     a.q, a.q_item_stride = _ptr(q), q_item_stride
     a.out, a.out_item_stride = _ptr(out), out_item_stride
@@ -392,6 +395,8 @@ def decode_args(k, v, n_q, n_kv, head_dim, max_tokens, q, out, *, n_items=1, ite
     a.norm_item_stride, a.norm_eps = norm_item_stride, norm_eps
     a.rope_cos, a.rope_sin = _ptr(rope_cos), _ptr(rope_sin)
     a.rope_item_stride = rope_item_stride
+    a._keep = (k, v, lens, q, out, k_new, v_new, q_norm, k_norm, rope_cos, rope_sin)  # noqa: SLF001
+    a._devices = frozenset(t.device.index for t in a._keep if t is not None and not isinstance(t, int))  # noqa: SLF001
     return a
 
 
@@ -416,7 +421,11 @@ def weights_args(weight, weight_out=None, *, item_stride=0, position=None, new_p
 
 def decode_weights(args: DecodeArgs, weights: WeightsArgs, workspace=None, stream=None) -> None:
     """tqk_decode_q8_weights: the decode, and each cached row's attention weight added to its running sum."""
-    _on_device(weights._device)  # noqa: SLF001
+    devices = args._devices | {d for d in (weights._device, _device_of(workspace)) if d is not None}  # noqa: SLF001
+    if len(devices) > 1:
+        raise ValueError(f"tensors of one call on several devices: {sorted(devices)}")
+    for d in devices:
+        _on_device(d)
     ws = _ptr(workspace) if workspace is not None else None
     nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     check(tqk_decode_q8_weights(ctypes.byref(args), ctypes.byref(weights), ws, nbytes, _stream(stream)),

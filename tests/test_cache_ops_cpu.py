@@ -237,3 +237,37 @@ def test_logit_clusters_fit_the_device(tmp_path):
         assert max(narrow) <= 8 and all(n == min(w, 8) for w, n in zip(wide, narrow))
     assert ctas((1, 128256, 148, 16), (37, 128256, 148, 16), (256, 128256, 148, 16), (512, 30001, 148, 16),
                 (512, 8001, 148, 16), (10, 30001, 148, 16), (7, 4096, 148, 16)) == [16, 8, 8, 2, 1, 8, 1]
+
+
+def test_decode_args_keep_and_check_their_tensors(tqk, monkeypatch):
+    """The struct holds bare addresses, so it keeps its tensors alive; a decode with weights refuses tensors of another
+    device wherever they are, and lengths that are not int32."""
+    import gc
+    import weakref
+
+    import torch
+    a = tqk.decode_args(_FakeTensor(1), _FakeTensor(1), 8, 2, 128, 64, _FakeTensor(1), _FakeTensor(1),
+                        lens=_FakeTensor(1, "int32"), k_new=_FakeTensor(1), v_new=_FakeTensor(1), q_norm=_FakeTensor(1),
+                        k_norm=_FakeTensor(1), rope_cos=_FakeTensor(1), rope_sin=_FakeTensor(1))
+    seen = [weakref.ref(t) for t in a._keep]
+    gc.collect()
+    assert len(seen) == 11 and all(r() is not None for r in seen)
+    del a
+    gc.collect()
+    assert all(r() is None for r in seen)
+    with pytest.raises(ValueError, match="int32"):
+        tqk.decode_args(FAKE, FAKE, 8, 2, 128, 64, FAKE, FAKE, lens=_FakeTensor(0, "int64"))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+
+    def call(decode_device, weights_device):
+        tqk.decode_weights(tqk.decode_args(FAKE, FAKE, 8, 2, 128, 64, FAKE, _FakeTensor(decode_device)),
+                           tqk.weights_args(_FakeTensor(weights_device)))
+
+    with pytest.raises(ValueError, match="several devices"):
+        call(1, 0)
+    with pytest.raises(ValueError, match="several devices"):
+        call(0, 1)
+    with pytest.raises(ValueError, match="cuda:1"):
+        call(1, 1)
+    with pytest.raises(ValueError, match="cuda:1"):
+        tqk.decode_weights(tqk.decode_args(FAKE, FAKE, 8, 2, 128, 64, FAKE, _FakeTensor(1)), tqk.weights_args(FAKE))
