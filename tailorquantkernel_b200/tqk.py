@@ -475,6 +475,13 @@ def _row_ptr(t, dtype: str):
     return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1], t.shape[0], t.shape[1]
 
 
+def _at_least(n: int, **arrays) -> None:
+    """Arrays that the kernel reads or writes n values of must hold them (addresses are taken as they are)."""
+    for name, t in arrays.items():
+        if t is not None and not isinstance(t, int) and t.numel() < n:
+            raise ValueError(f"{name} needs {n} values, got {t.numel()}")
+
+
 def logits_args(logits, *, out=None, choice=None, tokens=None, token_offsets=None, n_tokens=None, prompt_lens=None,
                 repetition=None, frequency=None, presence=None, bias_tokens=None, bias_values=None, bias_offsets=None,
                 n_bias=None, mask=None, mask_rows=None) -> LogitsArgs:
@@ -499,6 +506,11 @@ def logits_args(logits, *, out=None, choice=None, tokens=None, token_offsets=Non
         if words < (a.vocab_size + 31) // 32:
             raise ValueError("mask rows need a bit per token")
     a.mask_rows = _typed(mask_rows, "int32")
+    _at_least(a.n_rows, choice=choice, prompt_lens=prompt_lens, repetition=repetition, frequency=frequency,
+              presence=presence, mask_rows=mask_rows)
+    _at_least(a.n_rows + 1, token_offsets=token_offsets, bias_offsets=bias_offsets)
+    _at_least(a.n_tokens, tokens=tokens)
+    _at_least(a.n_bias, bias_tokens=bias_tokens, bias_values=bias_values)
     a._keep = (logits, out, choice, tokens, token_offsets, prompt_lens, repetition, frequency, presence,  # noqa: SLF001
                bias_tokens, bias_values, bias_offsets, mask, mask_rows)
     a._device = _device_of(*a._keep)  # noqa: SLF001

@@ -271,3 +271,41 @@ def test_decode_args_keep_and_check_their_tensors(tqk, monkeypatch):
         call(1, 1)
     with pytest.raises(ValueError, match="cuda:1"):
         tqk.decode_weights(tqk.decode_args(FAKE, FAKE, 8, 2, 128, 64, FAKE, _FakeTensor(1)), tqk.weights_args(FAKE))
+
+
+class _FakeMatrix(_FakeTensor):
+    """A fake CUDA tensor with a shape, contiguous."""
+
+    def __init__(self, *shape, dtype="float32"):
+        super().__init__(0, dtype)
+        self.shape = shape
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def stride(self, i):
+        return int(np.prod(self.shape[i + 1:]))
+
+
+def test_logits_args_refuse_arrays_that_are_too_short(tqk):
+    """Everything the kernel indexes by row or list entry is as long as the call says."""
+    i32 = dict(dtype="int32")
+    good = dict(out=_FakeMatrix(3, 64), choice=_FakeMatrix(3, **i32), tokens=_FakeMatrix(9, **i32),
+                token_offsets=_FakeMatrix(4, **i32), prompt_lens=_FakeMatrix(3, **i32), repetition=_FakeMatrix(3),
+                frequency=_FakeMatrix(3), presence=_FakeMatrix(3), bias_tokens=_FakeMatrix(5, **i32),
+                bias_values=_FakeMatrix(5), bias_offsets=_FakeMatrix(4, **i32), mask=_FakeMatrix(2, 2, **i32),
+                mask_rows=_FakeMatrix(3, **i32))
+    a = tqk.logits_args(_FakeMatrix(3, 64), **good)
+    assert (a.n_rows, a.vocab_size, a.n_tokens, a.n_bias, a.n_mask_rows) == (3, 64, 9, 5, 2)
+    for name in ("choice", "token_offsets", "prompt_lens", "repetition", "frequency", "presence", "bias_values", "bias_offsets",
+                 "mask_rows"):
+        short = _FakeMatrix(good[name].shape[0] - 1, dtype=str(good[name].dtype).split(".")[1])
+        with pytest.raises(ValueError, match=name):
+            tqk.logits_args(_FakeMatrix(3, 64), **{**good, name: short})
+    for name in ("n_tokens", "n_bias"):
+        with pytest.raises(ValueError, match="tokens"):
+            tqk.logits_args(_FakeMatrix(3, 64), **good, **{name: 10})
+    tqk.logits_args(_FakeMatrix(3, 64), tokens=_FakeMatrix(9, **i32), token_offsets=FAKE, repetition=FAKE)  # addresses
