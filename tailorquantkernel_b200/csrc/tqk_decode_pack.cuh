@@ -940,19 +940,12 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
         const int Tn = pre[n_items], Cn = min((int)gridDim.x, Tn);
         return (int)((long long)(blockIdx.x + 1) * Tn / Cn);
     };
-    if (WT != WT_NONE && warp == 0) {
-        // ahead of every wait: a CTA that gives up reaches none of its later units
-        for (int gt = g0; gt < g1;) {
-            const BalSeg sg = bal_segment(pre, lens, n_items, pairs, gt, g1);
-            if (sg.lt0 == 0 && lane < G) set_unfinished(p, sg.item, 2 * sg.pair * p.group + lane);
-            gt = sg.ubase + sg.lt1;
-        }
-    }
     int j = 0;  // ring position of the next tile
     for (int gt = g0;;) {
         {
             const BalSeg sg = bal_segment(pre, lens, n_items, pairs, gt, run_end());
             const bool do_append = p.k_new != nullptr && sg.lt1 == sg.tiles;  // the segment holding the last tile
+            if (WT != WT_NONE && sg.lt0 == 0 && tid < G) set_unfinished(p, sg.item, 2 * sg.pair * p.group + tid);
             pack_preamble<NB>(p, sg.item, 2 * sg.pair * p.group, 2 * sg.pair, sg.len - 1, do_append, warp, lane, qq,
                               qd, newrow, pro);
         }
@@ -995,7 +988,16 @@ __global__ void __launch_bounds__(PK_THREADS, TQK_PK_MINB) decode_q8_pack_bal_ke
         }
         if (timed_out) *timeout = 1;
         cta_sync<1, PK_WARPS * 32>();
-        if (*timeout) return;
+        if (*timeout) {
+            // the units from here on, which wait for this CTA's part for good
+            if (WT != WT_NONE && tid < G)
+                for (int u = gt; u < run_end();) {
+                    const BalSeg sg = bal_segment(pre, lens, n_items, pairs, u, run_end());
+                    set_unfinished(p, sg.item, 2 * sg.pair * p.group + tid);
+                    u = sg.ubase + sg.lt1;
+                }
+            return;
+        }
 
         pack_reduce<NB, L::RED_STRIDE, WT>(st, red, warp, g, t, tid);
         const int Tn = pre[n_items];
