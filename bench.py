@@ -1427,28 +1427,29 @@ def run_reference(args):
     if rank != 0:
         return 0  # the reference is a single-process CPU library: rank 0 alone runs it
     orc, kind = reference_oracle()
+    whose = "the reference's" if kind == "reference" else "the restated"
     gen_kind = reference_generator().kind
     shape = TINY[args.config] if args.tiny else {}
     if args.config == 7:
         wl = HostConfig7(orc, seed=7000, **shape)
         sec, n, threads = reference_forward_seconds(orc, wl, max(1, min(args.steps, 3)))
-        sample = (f"{n} tokens through the reference's tq_forward_token ending at position {wl.pos} (a context "
+        sample = (f"{n} tokens through {whose} tq_forward_token ending at position {wl.pos} (a context "
                   f"of 1 + {n} tokens minus one of 1 token, so set-up and cache fill cancel)")
     elif args.config == 6:
         wl = HostConfig6(orc, seed=6000, **shape)
         reference_layers_seconds(orc, wl, 0.0, max_tokens=1, min_tokens=1)
         sec, n, threads = reference_layers_seconds(orc, wl, args.ref_seconds, max_tokens=args.steps,
                                                    min_tokens=min(args.steps, 3))
-        sample = f"{n} whole tokens through the reference's attention_layer x {wl.L}, median per token"
+        sample = f"{n} whole tokens through {whose} attention_layer x {wl.L}, median per token"
     elif args.config == 5:
         wl = HostConfig5(orc, seed=5000, **shape)
         sec, n, threads = reference_prefill_token_seconds(orc, wl, args.ref_seconds)
-        sample = (f"{n} tokens: the first 32 tokens of the chunk through the reference's append + causal "
+        sample = (f"{n} tokens: the first 32 tokens of the chunk through {whose} append + causal "
                   f"attention, repeated, median per token")
     elif args.config == 3:
         wl = HostConfig3(orc, seed=3000, **shape)
         sec, n, threads = reference_ragged_seconds(orc, wl, args.ref_seconds)
-        sample = (f"{n} sequence-tokens of config 3 (the first 4 sequences through the reference's attend_q8), "
+        sample = (f"{n} sequence-tokens of config 3 (the first 4 sequences through {whose} attend_q8), "
                   f"median, scaled to the batch's mean length")
     else:
         wl = HostConfig2(orc, seed=1000, **shape) if args.config == 2 else HostConfig4(orc, seed=4000, **shape)
@@ -1475,6 +1476,9 @@ def run_reference(args):
             "hbm_gbs_equivalent": (wl.bytes_per_step / Config3.B if args.config == 3 else wl.bytes_per_step)
                                   / sec / 1e9 * (wl.n if args.config == 5 else 1),
             "e2e": {"value": value, "unit": "tokens/s", "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}}
+    if kind != "reference":
+        line["unavailable"] = ("no build of the reference here: what ran is this repository's scalar restatement of its CPU "
+                               "path, which is no measure of the reference's speed")
     print(json.dumps(line), flush=True)
     return 0
 

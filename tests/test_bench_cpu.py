@@ -125,3 +125,14 @@ def test_config_streams_tile_without_overlap():
     o = bench.config7_stream(L, nkv, hd, mt, hidden)
     check([(o["kv"](l, p, h), mt * hd) for l in range(L) for p in (0, 1) for h in range(nkv)] +
           [(o["norms"](l), 2 * hidden + 2 * hd) for l in range(L)] + [(o["final_norm"], hidden)])
+
+
+def test_reference_arm_says_when_the_reference_did_not_run():
+    """Without a build of the reference the restatement is timed, and the line says so instead of passing for the reference."""
+    import oracle
+    line = json.loads(_run("--impl", "reference", "--config", "7", "--tiny", "--steps", "2", "--warmup", "3",
+                           "--ref-seconds", "0.1")[0])
+    if oracle.available("ref_avx2"):
+        assert "unavailable" not in line and line["cpu_baseline"]["kind"] == "reference"
+    else:
+        assert "restatement" in line["unavailable"] and "the reference's" not in line["cpu_baseline"]["sample"]
