@@ -199,7 +199,8 @@ TQK_API int tqk_decode_workspace_size(const tqk_decode_args *a, size_t *bytes);
  * tickets at zero again, so calls of up to 16384 units (n_items x kv-head
  * units) can reuse it without re-initialising.  Zero it again before a call
  * with more units than any earlier one, and after a call that reported
- * TQK_ETIMEOUT.  Calls that share a workspace must be ordered on one stream.
+ * TQK_ETIMEOUT.  Calls that share a workspace must be ordered on one stream, from
+ * one host thread or several.
  * workspace == NULL uses a library-owned workspace per (device, stream; for
  * cudaStreamPerThread, whose handle is a stream of its own in every host thread,
  * also per thread), allocated on first use and kept, whose tickets live apart from

@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 
 #include "tqk_common.cuh"
 
@@ -27,6 +28,11 @@ struct DeviceInfo {
 };
 // Cached properties of the current device (initialised on first use).
 const DeviceInfo *device_info();
+
+// Held from where a decode takes its workspace (NULL: the library's for the stream) to its last launch: calls of several
+// host threads that share one follow one another, however many launches they have, and none grows a buffer that another
+// is about to launch with.
+std::unique_lock<std::mutex> workspace_lock(const void *workspace, cudaStream_t stream);
 
 // Library-owned decode partials buffer for (current device, stream; with
 // cudaStreamPerThread also the calling thread), grown on demand and zeroed when (re)allocated.  Returns nullptr on allocation failure.

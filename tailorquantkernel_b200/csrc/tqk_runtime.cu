@@ -7,6 +7,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <utility>
 
 namespace tqk {
 
@@ -25,6 +26,7 @@ std::map<StreamKey, Workspace> g_workspaces;
 std::map<StreamKey, Workspace> g_counters;
 std::map<StreamKey, Workspace> g_scratch;
 std::map<StreamKey, Workspace> g_prefill_stage;
+std::map<std::pair<const void *, StreamKey>, std::mutex> g_workspace_locks;  // entries stay, so that references do
 
 // Grows `w` to at least `bytes` (minimum 1 MiB), zeroing the new buffer on `stream`.  A buffer that a graph was captured
 // with is left to that graph for good when a larger one is needed; nothing grows while `stream` is captured.
@@ -99,6 +101,17 @@ int ensure_device() {
     if (n <= 0) return fail(TQK_ENODEV, "no CUDA device");
     if (!device_info()) return fail(TQK_ECUDA, "cannot initialise the current CUDA device");
     return TQK_OK;
+}
+
+std::unique_lock<std::mutex> workspace_lock(const void *workspace, cudaStream_t stream) {
+    int dev = -1;
+    if (!workspace && cudaGetDevice(&dev) != cudaSuccess) dev = -1;  // reported where the workspace is looked up
+    std::mutex *m;
+    {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        m = &g_workspace_locks[{workspace, workspace ? StreamKey{} : stream_key(dev, stream)}];
+    }
+    return std::unique_lock<std::mutex>(*m);
 }
 
 void *library_workspace(cudaStream_t stream, size_t bytes) {

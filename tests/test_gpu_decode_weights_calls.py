@@ -169,3 +169,48 @@ def test_short_caches_add_their_weights_in_the_decode(tqk, cuda, nq, nkv, hd, mt
     c.check(after)
     tqk.decode_weights(c.args(), c.wargs())
     assert torch.equal(_bits(c.dw), _bits(after)) and tqk.device_status() == 0
+
+
+@pytest.mark.parametrize("own_workspace", [False, True])
+def test_two_threads_on_one_stream(tqk, cuda, own_workspace):
+    """Calls of two host threads on one stream and one workspace: neither's decode comes between the other's decode and its
+    weight pass, and neither's growth takes the buffer that the other launches with."""
+    import threading
+    import torch
+    cases = [[Case(tqk, 121 + 10 * t + i, 8, 2, 128, n, [n], append=False) for i, n in enumerate((3000, 200, 800, 5000))]
+             for t in range(2)]
+    every = cases[0] + cases[1]
+    for c in every:
+        c.want = c.dw.clone()
+        tqk.decode_weights(c.args(64), c.wargs(c.want))
+        c.want_out = c.out.clone()
+        c.after = torch.full_like(c.dw, float("nan"))
+        c.plain = torch.empty_like(c.out)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    ws = torch.zeros(max(tqk.decode_weights_workspace_size(c.args(64)) for c in every), dtype=torch.uint8,
+                     device="cuda") if own_workspace else None
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(cs):
+        try:
+            for _ in range(50):
+                for c in cs:
+                    tqk.decode_weights(c.args(64), c.wargs(c.after), ws, stream=s)
+                    c.out, keep = c.plain, c.out
+                    tqk.decode(c.args(64), ws, stream=s)
+                    c.out = keep
+        except Exception as e:  # seen by the test
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(cs,)) for cs in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for c in every:
+        assert torch.equal(_bits(c.after), _bits(c.want)) and torch.equal(c.out, c.want_out)
+        assert (c.plain - c.want_out).abs().max() < 1e-5
