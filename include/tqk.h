@@ -231,7 +231,12 @@ TQK_API int tqk_decode_q8(const tqk_decode_args *a, void *workspace, size_t work
  *     tqk_decode_q8 if large enough); NULL = library-owned, per (device, stream).
  *   - One or two launches.  Under stream capture a caller workspace is required
  *     (TQK_EWORKSPACE otherwise): graphs that may run at the same time need one
- *     each. */
+ *     each.
+ *   - Only this call keeps sums.  A prompt that goes through tqk_prefill_q8 or the
+ *     batched calls leaves none: the caller sets its rows' sums (zeros, say; equal
+ *     sums are evicted by slot order) and positions, or feeds the prompt's last
+ *     tokens one by one through this call.  tqk_attention_layer appends without
+ *     touching the sums, so the appended row's slot would keep what it held. */
 typedef struct {
     const float *weight;         /* device, [n_kv][max_tokens] of item 0: the sums before the call */
     float *weight_out;           /* device, same layout: the sums after it; may be weight (the usual case), else
@@ -256,7 +261,10 @@ TQK_API int tqk_decode_q8_weights(const tqk_decode_args *a, const tqk_weights_ar
  * and position.  So rows move only as far as needed, and their order in the cache
  * is no longer that of the positions; attention does not depend on it (RoPE is
  * already in the K rows).  Afterwards the item has min(len_i, budget) rows
- * (lens_out); a next token is appended at that slot with its own position's RoPE.
+ * (lens_out); a next token is appended at that slot with its own position's RoPE:
+ * by tqk_decode_q8_weights or tqk_decode_q8, whose tables and lengths are given
+ * apart.  tqk_forward_token cannot go on with such a cache (its one position is
+ * the slot, the length and the row of the RoPE table).
  *   - Slots from min(len_i, budget) on are left as they were in every array.
  *   - weight_out / position_out may be weight / position (in place) or arrays of
  *     their own (which then receive every kept row's value); they must not

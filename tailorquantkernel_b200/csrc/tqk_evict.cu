@@ -14,8 +14,8 @@
 //      above every weight), into shared memory;
 //   2. the budget-th largest key by radix select, 11 + 11 + 10 bits: a histogram
 //      per CTA in shared memory, summed over the cluster through distributed
-//      shared memory, searched by every CTA alike.  The third digit only looks at
-//      the keys that share the first two, which the second pass lists;
+//      shared memory, searched by every CTA alike.  The second pass lists the keys
+//      that share the first digit, and the third only looks at those;
 //   3. each thread marks the holes (evicted, below `budget`) and movers (kept,
 //      from `budget` on) of its own run of consecutive slots; block and cluster
 //      prefix sums of their counts give every one its rank, and their slots go
@@ -51,7 +51,7 @@ static_assert(EV_CLUSTER_MAX * EV_THREADS * EV_RUN_MAX == TQK_EVICT_MAX_LEN, "do
 struct EvictParams {
     uint8_t *k, *v;
     long long item_stride;  // bytes
-    int n_kv, max_tokens;
+    int max_tokens;
     const int *lens;
     int len0, len_step, len_cap;
     int budget, n_first, n_recent;
@@ -73,7 +73,7 @@ struct EvictShared {
     int max_pos;                 // this CTA's largest position
     int counts[2];               // this CTA's holes and movers
     int ties;                    // this CTA's keys equal to the threshold
-    int n_close;                 // keys that share the first two digits
+    int n_close;                 // keys that share the first digit
     int found[3][3];             // per digit: the bin of the budget-th key, how many keys lie above it, its own
     int pre_h[EV_CLUSTER_MAX + 1], pre_m[EV_CLUSTER_MAX + 1];
 };
@@ -110,7 +110,7 @@ __device__ __forceinline__ int block_prefix(int v, int *warp_tot, int *total) {
 // One warp moves rows of both planes from slots src to slots dst, lane l's move in its src and dst, the first n lanes'.
 // A row is 9 16-byte units (9 words for head_dim 32), or twice as many; K's and V's units lie next to each other in the
 // lanes where both fit, so a lane's place in the row never changes and a move costs one load and one store.  Denser
-// layouts (every lane at work, twice the bytes in flight) were slower: 128 us against 118 us for a ragged batch.
+// layouts (every lane at work, twice the bytes in flight) were slower by 8% for a ragged batch.
 template <int NB>
 __device__ __forceinline__ void move_rows(uint8_t *kh, uint8_t *vh, int src, int dst, int n) {
     constexpr int ROW = NB * BLOCK_BYTES;
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(T, 1024 / T) evict_kernel(const EvictParams p)
     //         them are kept
     uint32_t prefix = 0;
     int need = budget, equal = 0;
-    uint32_t *close = reinterpret_cast<uint32_t *>(pos_s);  // the keys that share two digits, as far as they fit
+    uint32_t *close = reinterpret_cast<uint32_t *>(pos_s);  // the keys that share the first digit, as far as they fit
     const int close_cap = staged ? T * p.run : 0;
 #pragma unroll
     for (int digit = 0; digit < 3; digit++) {
@@ -495,7 +495,6 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
         p.k = reinterpret_cast<uint8_t *>(a->k);
         p.v = reinterpret_cast<uint8_t *>(a->v);
         p.item_stride = a->item_stride * BLOCK_BYTES;
-        p.n_kv = a->n_kv_heads;
         p.max_tokens = a->max_tokens;
         p.lens = a->lens;
         p.len0 = a->len0;
@@ -522,9 +521,10 @@ extern "C" int tqk_evict_q8(const tqk_evict_args *a, tqk_stream_t stream) {
             cluster *= 2;
         // Moving many rows keeps the SMs that do it busy for longer than finding them.  Where SMs are left over and the
         // sums and positions go elsewhere (a cluster may still read them when another is done), several clusters share
-        // a head's moves, each finding them for itself.  Half of 131072 rows kept, with one cluster per head and so: 1
-        // head 66 and 33 us, 2 heads 69 and 46 us, 4 heads 72 and 60 us.  Only up to half of the SMs: 16 clusters of 8
-        // do not all run at once (8 heads: 85 and 123 us; 8 clusters of 16 CTAs do not either: 112 us)
+        // a head's moves, each finding them for itself.  Half of 131072 rows kept, in place (one cluster per head) and
+        // elsewhere (so): 1 head 61 and 33 us, 2 heads 63 and 39 us, 4 heads 65 and 53 us.  Only up to half of the SMs:
+        // 16 clusters of 8 do not all run at once (8 heads, at the time 85 us with 8 clusters: 123 us; 8 clusters of 16
+        // CTAs do not either: 112 us)
         int parts = 1;
         const long long busy = units * cluster;
         const int moves = a->budget < max_len - a->budget ? a->budget : max_len - a->budget;  // at most, at max_len

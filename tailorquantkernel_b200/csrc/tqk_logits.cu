@@ -6,7 +6,9 @@
 // CTAs in turn.  The bulk of a row -- tokens in neither its history nor its bias
 // list -- only meets the mask and is streamed through registers: 8 16-byte loads
 // in flight per thread, each logit read and written once, which is the kernel's
-// floor (8 bytes of DRAM traffic per token).  Around the stream:
+// floor (8 bytes of DRAM traffic per token).  256 rows of 128256 tokens take 48 us
+// with a mask alone (floor 41) and 112 us with histories of 500 to 16000 and biases,
+// where issue slots bound it (60% busy).  Around the stream:
 //   * while the first logits are on their way, every CTA scans the history and
 //     counts its own tokens in shared memory (a counter per token: seen, in the
 //     bias list, and the count after the prompt; integer atomics, so their order
@@ -14,10 +16,9 @@
 //     ids in many vocabularies; dealing out small blocks spreads them over the CTAs;
 //   * the stream reads the bitmap like a second mask; each warp then lists its
 //     marked tokens, fetches their logits again (ahead of the next logits of the
-//     stream, or they would queue behind those: 256 rows 137 us with loads where they
-//     are used, 130 us so) and works the list off with all lanes, so the division and
-//     the branches of the penalties cost by the distinct tokens of the history, not
-//     by the vocabulary;
+//     stream, or they would queue behind those: 5% of the time with histories) and
+//     works the list off with all lanes, so the division and the branches of the
+//     penalties cost by the distinct tokens of the history, not by the vocabulary;
 //   * each CTA pushes its candidate for the greedy choice to the first CTA's
 //     shared memory; a cluster barrier later the first CTA compares them.
 #include "tqk_internal.h"
@@ -42,8 +43,8 @@ constexpr int LG_STAGE = 2 * LG_SCAN;                    // ... and the next one
 static_assert(LG_STAGE == LG_WARPS * LG_LIST, "the listed logits take the staging's memory");
 // Counters: 16 bits per token (two to a word) for histories with up to LG_SHORT entries behind the prompt, else 32 bits.
 // From the top: seen, in the bias list, more than once in the bias list, and the count after the prompt.  The width is
-// a value of the row, not of the type: two copies of the row's work in one kernel miss the instruction cache (256 rows
-// of 128256 tokens: 75 us with both, 67 us with one).
+// a value of the row, not of the type: two copies of the row's work in one kernel miss the instruction cache (12% slower
+// with short histories).
 constexpr int LG_SHORT = (1 << 13) - 1;
 constexpr int LG_COUNT_MAX = (1 << 29) - 1;
 struct Counters {
@@ -209,7 +210,7 @@ __device__ __forceinline__ void mark_shared(bool go, uint32_t word, uint32_t uni
 // 1024 on their way, so that they take no registers beside the logits.  What bounds this is the instructions issued,
 // every CTA of the row looking at every entry (256 rows: 68 M warp instructions, 16 M without histories): each lane
 // updates its own entries, one in C active, without a branch.  Collecting the CTA's entries first, to update them with
-// all lanes, takes more of them (256 rows 130 us, 121 us so).
+// all lanes, takes more of them (7% slower).
 __device__ __forceinline__ void count_history(const LogitsParams &p, const Row &r, int c0, uint32_t *bitmap, uint32_t *lists) {
     const Counters &k = r.counters;
     const int tid = threadIdx.x;
