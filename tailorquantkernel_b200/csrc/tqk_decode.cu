@@ -1280,7 +1280,7 @@ int decode_impl(const tqk_decode_args *a, const tqk_gather_dst *gd, void *worksp
     float *part = nullptr;
     std::unique_lock<std::mutex> lock;
     if (need) {
-        lock = workspace_lock(workspace, st);
+        if (!lock_workspace(workspace, st, lock)) return fail(TQK_ECUDA, "decode: cannot lock the workspace");
         if (!workspace) {
             // library-owned: tickets in a buffer of their own, which partials never touch
             counters = library_counters(st, pl.counters_bytes);
@@ -1377,7 +1377,8 @@ extern "C" int tqk_decode_q8_weights(const tqk_decode_args *a, const tqk_weights
     const WeightScratch ws = weight_scratch(a, pl);
     cudaStream_t st = (cudaStream_t)stream;
     // the weight pass reads what the decode leaves in the workspace: no other call of the stream in between
-    const std::unique_lock<std::mutex> lock = workspace_lock(workspace, st);
+    std::unique_lock<std::mutex> lock;
+    if (!lock_workspace(workspace, st, lock)) return fail(TQK_ECUDA, "tqk_decode_q8_weights: cannot lock the workspace");
     int *counters = nullptr;
     uint8_t *base = nullptr;  // where ws's offsets from part_off on count from
     if (!workspace) {

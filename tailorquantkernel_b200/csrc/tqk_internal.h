@@ -31,8 +31,8 @@ const DeviceInfo *device_info();
 
 // Held from where a decode takes its workspace (NULL: the library's for the stream) to its last launch: calls of several
 // host threads that share one follow one another, however many launches they have, and none grows a buffer that another
-// is about to launch with.
-std::unique_lock<std::mutex> workspace_lock(const void *workspace, cudaStream_t stream);
+// is about to launch with.  false: no lock could be had.
+bool lock_workspace(const void *workspace, cudaStream_t stream, std::unique_lock<std::mutex> &held);
 
 // Library-owned decode partials buffer for (current device, stream; with
 // cudaStreamPerThread also the calling thread), grown on demand and zeroed when (re)allocated.  Returns nullptr on allocation failure.

@@ -5,6 +5,7 @@
 
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <map>
 #include <mutex>
 #include <utility>
@@ -57,6 +58,17 @@ void *grow_zeroed(Workspace &w, cudaStream_t stream, size_t bytes) {
     w.captured = capturing != cudaStreamCaptureStatusNone;
     return w.ptr;
 }
+
+void *library_buffer(std::map<StreamKey, Workspace> &buffers, cudaStream_t stream, size_t bytes) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    try {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        return grow_zeroed(buffers[stream_key(dev, stream)], stream, bytes);
+    } catch (const std::exception &) {  // no exception may leave a C entry
+        return nullptr;
+    }
+}
 }  // namespace
 
 int fail(int status, const char *msg) {
@@ -103,44 +115,31 @@ int ensure_device() {
     return TQK_OK;
 }
 
-std::unique_lock<std::mutex> workspace_lock(const void *workspace, cudaStream_t stream) {
+bool lock_workspace(const void *workspace, cudaStream_t stream, std::unique_lock<std::mutex> &held) {
     int dev = -1;
-    if (!workspace && cudaGetDevice(&dev) != cudaSuccess) dev = -1;  // reported where the workspace is looked up
-    std::mutex *m;
-    {
-        std::lock_guard<std::mutex> lock(g_mutex);
-        m = &g_workspace_locks[{workspace, workspace ? StreamKey{} : stream_key(dev, stream)}];
+    if (!workspace && cudaGetDevice(&dev) != cudaSuccess) return false;
+    try {
+        std::mutex *m;
+        {
+            std::lock_guard<std::mutex> lock(g_mutex);
+            m = &g_workspace_locks[{workspace, workspace ? StreamKey{} : stream_key(dev, stream)}];
+        }
+        held = std::unique_lock<std::mutex>(*m);
+    } catch (const std::exception &) {  // no exception may leave a C entry
+        return false;
     }
-    return std::unique_lock<std::mutex>(*m);
+    return true;
 }
 
-void *library_workspace(cudaStream_t stream, size_t bytes) {
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-    std::lock_guard<std::mutex> lock(g_mutex);
-    return grow_zeroed(g_workspaces[stream_key(dev, stream)], stream, bytes);
-}
+void *library_workspace(cudaStream_t stream, size_t bytes) { return library_buffer(g_workspaces, stream, bytes); }
 
 int *library_counters(cudaStream_t stream, size_t bytes) {
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-    std::lock_guard<std::mutex> lock(g_mutex);
-    return static_cast<int *>(grow_zeroed(g_counters[stream_key(dev, stream)], stream, bytes));
+    return static_cast<int *>(library_buffer(g_counters, stream, bytes));
 }
 
-void *library_scratch(cudaStream_t stream, size_t bytes) {
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-    std::lock_guard<std::mutex> lock(g_mutex);
-    return grow_zeroed(g_scratch[stream_key(dev, stream)], stream, bytes);
-}
+void *library_scratch(cudaStream_t stream, size_t bytes) { return library_buffer(g_scratch, stream, bytes); }
 
-void *library_prefill_stage(cudaStream_t stream, size_t bytes) {
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
-    std::lock_guard<std::mutex> lock(g_mutex);
-    return grow_zeroed(g_prefill_stage[stream_key(dev, stream)], stream, bytes);
-}
+void *library_prefill_stage(cudaStream_t stream, size_t bytes) { return library_buffer(g_prefill_stage, stream, bytes); }
 
 }  // namespace tqk
 
