@@ -1383,9 +1383,7 @@ extern "C" int tqk_decode_q8_weights(const tqk_decode_args *a, const tqk_weights
     uint8_t *base = nullptr;  // where ws's offsets from part_off on count from
     if (!workspace) {
         // two graphs captured on one stream would share its buffers and may be replayed at the same time
-        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(st, &capturing) != cudaSuccess) (void)cudaGetLastError();
-        if (capturing != cudaStreamCaptureStatusNone)
+        if (stream_captures(st))
             return fail(TQK_EWORKSPACE, "tqk_decode_q8_weights: a call under stream capture needs a workspace of its own");
         // library-owned: tickets in a buffer of their own, which scores and partials never touch
         counters = library_counters(st, ws.ticket_bytes);

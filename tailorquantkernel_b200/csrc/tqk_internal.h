@@ -20,6 +20,9 @@ int check_launch(const char *what);
 // Makes sure a CUDA device is usable from this thread; TQK_ENODEV otherwise.
 int ensure_device();
 
+// Whether work on `stream` goes into a graph under capture.
+bool stream_captures(cudaStream_t stream);
+
 struct DeviceInfo {
     int device = -1;
     int sm_count = 0;

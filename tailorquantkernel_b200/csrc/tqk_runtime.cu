@@ -32,14 +32,13 @@ std::map<std::pair<const void *, StreamKey>, std::mutex> g_workspace_locks;  // 
 // Grows `w` to at least `bytes` (minimum 1 MiB), zeroing the new buffer on `stream`.  A buffer that a graph was captured
 // with is left to that graph for good when a larger one is needed; nothing grows while `stream` is captured.
 void *grow_zeroed(Workspace &w, cudaStream_t stream, size_t bytes) {
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess) (void)cudaGetLastError();
+    const bool capturing = stream_captures(stream);
     if (w.bytes >= bytes && w.ptr) {
-        if (capturing != cudaStreamCaptureStatusNone) w.captured = true;
+        if (capturing) w.captured = true;
         return w.ptr;
     }
     if (w.ptr) {
-        if (capturing != cudaStreamCaptureStatusNone) return nullptr;
+        if (capturing) return nullptr;
         if (!w.captured) {
             // the old buffer may still be in use by work queued on `stream`
             cudaStreamSynchronize(stream);
@@ -55,7 +54,7 @@ void *grow_zeroed(Workspace &w, cudaStream_t stream, size_t bytes) {
     }
     if (cudaMemsetAsync(w.ptr, 0, grow, stream) != cudaSuccess) return nullptr;
     w.bytes = grow;
-    w.captured = capturing != cudaStreamCaptureStatusNone;
+    w.captured = capturing;
     return w.ptr;
 }
 
@@ -70,6 +69,16 @@ void *library_buffer(std::map<StreamKey, Workspace> &buffers, cudaStream_t strea
     }
 }
 }  // namespace
+
+bool stream_captures(cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) {
+        // the legacy stream while another stream is captured: the status says nothing, and that capture goes on
+        (void)cudaGetLastError();
+        return false;
+    }
+    return status != cudaStreamCaptureStatusNone;
+}
 
 int fail(int status, const char *msg) {
     std::snprintf(t_last_error, sizeof t_last_error, "%s", msg);

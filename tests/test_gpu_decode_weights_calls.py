@@ -214,3 +214,25 @@ def test_two_threads_on_one_stream(tqk, cuda, own_workspace):
     for c in every:
         assert torch.equal(_bits(c.after), _bits(c.want)) and torch.equal(c.out, c.want_out)
         assert (c.plain - c.want_out).abs().max() < 1e-5
+
+
+def test_a_capture_elsewhere_does_not_matter(tqk, cuda):
+    """While a stream that does not follow the default stream is captured, a call with the library's workspace on another
+    stream goes ahead, growth included, and the capture goes on."""
+    import torch
+    c = Case(tqk, 141, 8, 2, 128, 700, [700], append=False)
+    want = c.dw.clone()
+    tqk.decode_weights(c.args(64), c.wargs(want))
+    after = torch.full_like(c.dw, float("nan"))
+    torch.cuda.synchronize()
+    s, other, g, x = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.zeros(1, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s, capture_error_mode="relaxed"):
+        x.add_(1)
+        tqk.decode_weights(c.args(64), c.wargs(after), stream=other)
+        x.add_(1)
+    torch.cuda.synchronize()
+    assert torch.equal(_bits(after), _bits(want))
+    g.replay()
+    torch.cuda.synchronize()
+    assert x.item() == 2
