@@ -21,6 +21,7 @@ work goes through libtqk's C ABI (tailorquantkernel_b200.tqk).
 """
 from __future__ import annotations
 
+import atexit
 from typing import List, Sequence, Tuple
 
 TILE_TOKENS = 64  # the decode kernels' tile: ranges start on tile boundaries
@@ -106,6 +107,14 @@ def batch_shard(lens: Sequence[int], world: int) -> List[List[int]]:
     return [sorted(o) for o in owned]
 
 
+def _leave_group():
+    """At exit: a process that ends inside a gloo group may be aborted by the group's own threads, above all after a failed
+    collective, instead of ending with its own exit code."""
+    import torch.distributed as dist
+    if dist.is_initialized():
+        dist.destroy_process_group()
+
+
 def gather_partials(dist, local, group=None):
     """All-gathers each rank's partial records (a contiguous tensor of the same
     shape on every rank) into one [world, *local.shape] tensor, rank order."""
@@ -113,6 +122,8 @@ def gather_partials(dist, local, group=None):
     world = dist.get_world_size(group)
     out = torch.empty((world,) + tuple(local.shape), dtype=local.dtype, device=local.device)
     if dist.get_backend(group) == "gloo":  # host ranks (tests): list form
+        atexit.unregister(_leave_group)  # once
+        atexit.register(_leave_group)
         dist.all_gather(list(out.unbind(0)), local.contiguous(), group=group)
     else:
         dist.all_gather_into_tensor(out, local.contiguous(), group=group)
